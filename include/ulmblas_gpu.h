@@ -493,6 +493,79 @@ int ulmblas_gpu_dgetrf_static(int m, int n, double *dA, int ldA, int *dPiv,
 int ulmblas_gpu_dlaswp(int n, double *dA, int ldA, int k1, int k2,
                        const int *dPiv, int incPiv, void *stream);
 
+/* Softmax cross entropy of a classifier (no counterpart in the reference: a
+ * product whose result is reduced in its epilogue).  W is hidden x vocab and X
+ * hidden x tokens, column-major: a column of W is one row of the classifier, a
+ * column of X one token's hidden state.  For every token t whose label
+ * dLabel[t] is a column of W (0 .. vocab-1) and not `ignore`, with
+ * z = alpha * W^T x_t:
+ *     dLse[t]  = log sum_v exp(z_v)
+ *     dLoss[t] = dLse[t] - z_label
+ * Both are 0 for any other token, whose column of X is not computed with,
+ * whatever it holds.  s: fp32 operands; b: bf16 operands (their 16 bits), sums
+ * and results in fp32.  The logits are not kept.  `work`: device memory of
+ * ulmblas_gpu_?xent_worksize(hidden, tokens, vocab) bytes, 16-byte aligned, any
+ * contents, for one call at a time.  hidden at most 2^20, tokens and vocab at
+ * most 2^28 (worksize 0, BAD_ARGUMENT beyond that); tokens == 0 does nothing.
+ * Everything is enqueued on `stream`, on the current device; nothing is
+ * allocated or synchronised.  The same call gives the same bits. */
+long ulmblas_gpu_sxent_worksize(int hidden, int tokens, int vocab);
+long ulmblas_gpu_bxent_worksize(int hidden, int tokens, int vocab);
+int ulmblas_gpu_sxent(int hidden, int tokens, int vocab, float alpha,
+                      const float *dW, int ldW, const float *dX, int ldX,
+                      const int *dLabel, int ignore, float *dLoss, float *dLse,
+                      void *work, void *stream);
+int ulmblas_gpu_bxent(int hidden, int tokens, int vocab, float alpha,
+                      const unsigned short *dW, int ldW,
+                      const unsigned short *dX, int ldX, const int *dLabel,
+                      int ignore, float *dLoss, float *dLse, void *work,
+                      void *stream);
+/* The gradient of the above.  dLse is what the forward call returned, dGLoss
+ * and dGLse (null: zero) the gradients of its two results; with
+ *     P_vt = dGLoss[t] (exp(z_vt - dLse[t]) - [v = label]) + dGLse[t] exp(z_vt - dLse[t])
+ * for tokens with a target and 0 for others,
+ *     gX = alpha * W * P            (hidden x tokens; whole columns are written)
+ *     gW = alpha * X * P^T + beta * gW      (hidden x vocab)
+ * beta == 0 never reads gW.  A null dGW or dGX is not computed.  The logits are
+ * computed again, a piece of the vocabulary at a time, and P of that piece is
+ * rounded to the operands' type for the two products.  Outputs must not overlap
+ * inputs, each other or `work` (ulmblas_gpu_?xent_grad_worksize bytes). */
+long ulmblas_gpu_sxent_grad_worksize(int hidden, int tokens, int vocab);
+long ulmblas_gpu_bxent_grad_worksize(int hidden, int tokens, int vocab);
+int ulmblas_gpu_sxent_grad(int hidden, int tokens, int vocab, float alpha,
+                           const float *dW, int ldW, const float *dX, int ldX,
+                           const int *dLabel, int ignore, const float *dLse,
+                           const float *dGLoss, const float *dGLse, float beta,
+                           float *dGW, int ldGW, float *dGX, int ldGX,
+                           void *work, void *stream);
+int ulmblas_gpu_bxent_grad(int hidden, int tokens, int vocab, float alpha,
+                           const unsigned short *dW, int ldW,
+                           const unsigned short *dX, int ldX, const int *dLabel,
+                           int ignore, const float *dLse, const float *dGLoss,
+                           const float *dGLse, float beta, unsigned short *dGW,
+                           int ldGW, unsigned short *dGX, int ldGX, void *work,
+                           void *stream);
+
+/* nrm2 and scal over a group of tensors, such as all gradients of a model.
+ * Tensor i is n[i] consecutive elements of type[i] ('s': fp32, 'b': bf16) from
+ * dX[i] on, aligned to its elements; the three lists are host memory, read
+ * before the call returns.  n[i] at most 2^40.
+ * gnrm2: *dNorm = the Euclidean norm of all elements together (squares and
+ * sums in fp64, so nothing overflows or underflows on the way; 0 for an empty
+ * group).  `work`: device memory of ulmblas_gpu_gnrm2_worksize(count) bytes,
+ * 8-byte aligned, any contents, for one call at a time.
+ * gclip: dY[i] = dX[i] * min(1, largest / *dNorm), elementwise, dNorm on the
+ * device; dY[i] is dX[i] itself or does not overlap any tensor of the group.
+ * A norm that is infinite or no number leaves the values as they are.  Nothing
+ * is allocated or synchronised; the same call gives the same bits. */
+long ulmblas_gpu_gnrm2_worksize(int count);
+int ulmblas_gpu_gnrm2(int count, const char *type, const long *n,
+                      const void *const *dX, float *dNorm, void *work,
+                      void *stream);
+int ulmblas_gpu_gclip(int count, const char *type, const long *n,
+                      const void *const *dX, void *const *dY,
+                      const float *dNorm, float largest, void *stream);
+
 /* Selects the workgroup-tile variant the next launches use: 0 = automatic
  * choice from the shape (default), otherwise one of the ids listed by
  * ulmblas_gpu_variant_name().  For tuning and tests; returns
@@ -543,6 +616,9 @@ int ulmblas_gpu_set_variant(int precision /* 'd' or 's' */, int variant);
  *                     any-shape kernel alone over the triangle; 4, 5: as 1, 2
  *                     with the second largest tile (blocks of its order) for
  *                     the square;
+ *  XENT_PIECE         value > 0: the gradient of the cross entropy takes at most
+ *                     this many columns of W (rounded up to 256) at a time; 0
+ *                     (default): as many as the workspace's bound allows;
  *  FAIL_ALLOC         the next `value` device allocations of the host entry
  *                     points fail (as if the device were out of memory).
  * Every kernel runs to its end whatever is set here. */
@@ -557,7 +633,8 @@ enum ULMBLAS_GPU_TEST {
     ULMBLAS_GPU_TEST_LU_SIMPLE_PANELS = 8,
     ULMBLAS_GPU_TEST_TRSM_PARTS = 9,
     ULMBLAS_GPU_TEST_HOST_HEAD = 10,
-    ULMBLAS_GPU_TEST_TRI_WAY = 11
+    ULMBLAS_GPU_TEST_TRI_WAY = 11,
+    ULMBLAS_GPU_TEST_XENT_PIECE = 12
 };
 int ulmblas_gpu_test_control(int what, long value);
 /* How ulmblas_gpu_dgemm / _sgemm (precision 'd' / 's') would launch an

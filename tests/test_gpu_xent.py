@@ -1,0 +1,311 @@
+"""Softmax cross entropy of a classifier and its gradient on the GPU against a plain implementation in 64 bits, within
+bounds that follow from the arithmetic (xent_ref)."""
+import numpy as np
+import pytest
+
+import xent_ref
+from ulmblas_amd import blas
+
+pytestmark = pytest.mark.gpu
+
+IGNORE = -100
+
+
+def window(A, prec, pad, off, fill=float("nan")):
+    """A [rows, cols] matrix as a device window with row stride cols + pad, `off` elements into its memory; the
+    memory around it holds `fill`.  Returns (tensor of the window, its 64-bit values, stride)."""
+    import torch
+    dt = {"s": torch.float32, "b": torch.bfloat16}[prec]
+    rows, cols = A.shape
+    ld = cols + pad
+    flat = torch.full((off + rows * ld + 64,), fill, dtype=dt, device="cuda")
+    view = flat[off:off + rows * ld].view(rows, ld)[:, :cols]
+    view.copy_(torch.from_numpy(A).to(dt))
+    return view, view.double().cpu().numpy(), ld
+
+
+class Problem:
+    def __init__(self, prec, hidden, tokens, vocab, pad=0, off=0, alpha=1.0, masked=0.0, seed=0, spread=1.5):
+        import torch
+        rng = np.random.default_rng(seed)
+        W = rng.standard_normal((vocab, hidden)) * (2.0 / np.sqrt(hidden))
+        label = rng.integers(0, vocab, tokens)
+        X = rng.standard_normal((tokens, hidden)) + spread * W[label]
+        drop = rng.random(tokens) < masked
+        label[drop] = np.resize(np.array([IGNORE, -1, vocab, 2 ** 31 - 1, -2 ** 31]), int(drop.sum()))
+        X[drop] = np.resize(np.array([np.nan, np.inf, -np.inf, 1.0]), (int(drop.sum()), 1))
+        self.prec, self.H, self.T, self.V, self.alpha = prec, hidden, tokens, vocab, alpha
+        self.label = label
+        self.W, self.w64, self.ldW = window(W, prec, pad, off)
+        self.X, self.x64, self.ldX = window(X, prec, pad, off)
+        self.dlabel = torch.from_numpy(label.astype(np.int32)).cuda()
+        self.gloss = (rng.standard_normal(tokens) / max(tokens, 1)).astype(np.float32)
+        self.glse = (rng.standard_normal(tokens) * 0.1 / max(tokens, 1)).astype(np.float32)
+        self.rng = rng
+
+    def work(self, size):
+        """A workspace whose every word is NaN."""
+        import torch
+        return torch.full((size,), 0xff, dtype=torch.uint8, device="cuda")
+
+    def forward(self, stream=None):
+        import torch
+        loss, lse = (torch.full((self.T + 3,), 7.5, device="cuda") for _ in range(2))
+        work = self.work(blas.xent_worksize(self.prec, self.H, self.T, self.V))
+        blas.gpu_xent(self.prec, self.H, self.T, self.V, self.alpha, self.W, self.ldW, self.X, self.ldX, self.dlabel,
+                      IGNORE, loss, lse, work=work, stream=stream)
+        torch.cuda.synchronize()
+        assert (loss[self.T:] == 7.5).all() and (lse[self.T:] == 7.5).all()
+        return loss[:self.T].double().cpu().numpy(), lse[:self.T].double().cpu().numpy()
+
+    def check_forward(self):
+        loss, lse = self.forward()
+        x64 = np.where(xent_ref.valid(self.label, self.V, IGNORE)[:, None], self.x64, 0.0)
+        wloss, wlse, blse, bloss = xent_ref.forward(self.w64, x64, self.label, self.alpha, IGNORE, self.prec)
+        assert np.isfinite(loss).all() and np.isfinite(lse).all()
+        assert (np.abs(lse - wlse) <= blse).all(), np.nanmax(np.abs(lse - wlse) / blse)
+        assert (np.abs(loss - wloss) <= bloss).all(), np.nanmax(np.abs(loss - wloss) / bloss)
+        return lse
+
+    def check_backward(self, glse=True, beta=0.0, want=("W", "X"), pad_out=0, off_out=0):
+        import torch
+        x64 = np.where(xent_ref.valid(self.label, self.V, IGNORE)[:, None], self.x64, 0.0)
+        lse = xent_ref.forward(self.w64, x64, self.label, self.alpha, IGNORE, self.prec)[1].astype(np.float32)
+        gW0 = self.rng.standard_normal((self.V, self.H)) if beta else np.full((self.V, self.H), np.nan)
+        gW, gW64, ldGW = window(gW0, self.prec, pad_out, off_out, 3.25)
+        gX, _, ldGX = window(np.full((self.T, self.H), np.nan), self.prec, pad_out, off_out, 3.25)
+        work = self.work(blas.xent_grad_worksize(self.prec, self.H, self.T, self.V))
+        # rows without a target may hold anything here too
+        has = xent_ref.valid(self.label, self.V, IGNORE)
+        f = [torch.from_numpy(np.where(has, a, np.float32(np.nan))).cuda() for a in (lse, self.gloss, self.glse)]
+        blas.gpu_xent_grad(self.prec, self.H, self.T, self.V, self.alpha, self.W, self.ldW, self.X, self.ldX, self.dlabel,
+                           IGNORE, f[0], f[1], f[2] if glse else None, beta, gW if "W" in want else None, ldGW,
+                           gX if "X" in want else None, ldGX, work=work)
+        torch.cuda.synchronize()
+        wW, wX, bW, bX = xent_ref.backward(self.w64, x64, self.label, self.alpha, IGNORE, lse.astype(np.float64),
+                                           self.gloss.astype(np.float64),
+                                           self.glse.astype(np.float64) if glse else None, self.prec, beta,
+                                           gW64 if beta else None)
+        for name, got, want64, bound in (("W", gW, wW, bW), ("X", gX, wX, bX)):
+            g = got.double().cpu().numpy()
+            if name not in want:
+                assert np.isnan(g).all() or beta, name
+                continue
+            assert np.isfinite(g).all(), name
+            d = np.abs(g - want64)
+            assert (d <= bound).all(), (name, float((d / bound).max()))
+            # the memory around the window is as it was
+            flat = got.untyped_storage()
+            whole = torch.empty(0, dtype=got.dtype, device="cuda").set_(flat)
+            inside = torch.zeros_like(whole, dtype=torch.bool)
+            torch.as_strided(inside, got.shape, got.stride(), got.storage_offset())[:] = True
+            assert (whole[~inside] == 3.25).all(), name
+        if "X" in want:
+            assert (gX.double().cpu().numpy()[~has] == 0).all()
+        return gW, gX
+
+
+SIZES = [  # hidden, tokens, vocab
+    (1, 1, 1), (8, 1, 2), (64, 1, 1000), (65, 7, 257), (96, 16, 300), (72, 17, 4097), (200, 33, 640), (1000, 130, 777),
+    (512, 300, 5000), (40, 257, 511), (4097, 3, 130),
+]
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+@pytest.mark.parametrize("hidden,tokens,vocab", SIZES)
+def test_sizes(prec, hidden, tokens, vocab):
+    p = Problem(prec, hidden, tokens, vocab, seed=hidden + tokens)
+    p.check_forward()
+    p.check_backward()
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+def test_large_tiles(prec):
+    """Sizes that take the 256 x 256 tile in every product."""
+    p = Problem(prec, 128, 300, 26000, seed=5, masked=0.1)
+    p.check_forward()
+    p.check_backward()
+    q = Problem(prec, 1800, 6500, 1900, seed=6, masked=0.5)
+    q.check_forward()
+    q.check_backward()
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+@pytest.mark.parametrize("pad,off", [(1, 0), (0, 1), (8, 8), (3, 5)])
+def test_strides_and_alignment(prec, pad, off):
+    for hidden, tokens, vocab in ((128, 5, 515), (136, 140, 700)):
+        p = Problem(prec, hidden, tokens, vocab, pad=pad, off=off, alpha=0.7, masked=0.3, seed=pad * 10 + off)
+        p.check_forward()
+        p.check_backward(pad_out=pad, off_out=off, beta=0.5)
+        p.check_backward(pad_out=0, off_out=0)
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+@pytest.mark.parametrize("tokens", [1, 6, 150, 1100])
+@pytest.mark.parametrize("masked", [0.5, 0.97, 1.0])
+def test_rows_without_a_target(prec, tokens, masked):
+    """Labels that are `ignore`, negative or past the vocabulary; those rows of X, lse and the gradients hold NaN and
+    infinities, and nothing of it reaches a result."""
+    p = Problem(prec, 104, tokens, 900, masked=masked, seed=tokens)
+    p.check_forward()
+    p.check_backward()
+    p.check_backward(beta=0.75)
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+def test_ignore_may_be_a_row_of_the_classifier(prec):
+    import torch
+    p = Problem(prec, 64, 40, 50, seed=9)
+    label = p.label.copy()
+    label[::3] = 7
+    p.dlabel = torch.from_numpy(label.astype(np.int32)).cuda()
+    loss, lse = blas.gpu_xent(prec, p.H, p.T, p.V, 1.0, p.W, p.ldW, p.X, p.ldX, p.dlabel, 7)
+    got = loss.double().cpu().numpy()
+    want, _, _, bound = xent_ref.forward(p.w64, p.x64, label, 1.0, 7, prec)
+    assert (got[label == 7] == 0).all() and (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+@pytest.mark.parametrize("tokens", [3, 140])
+def test_pieces_of_the_vocabulary(prec, tokens):
+    p = Problem(prec, 200, tokens, 1500, seed=11, masked=0.2)
+    q = Problem(prec, 200, tokens, 1500, pad=1, seed=12, masked=0.2)        # packed
+    blas.test_control(blas.TEST_XENT_PIECE, 256)
+    try:
+        for x in (p, q):
+            x.check_forward()
+            x.check_backward(beta=0.5)
+            x.check_backward(glse=False, want=("X",))
+            x.check_backward(want=("W",))
+    finally:
+        blas.test_control(blas.TEST_XENT_PIECE, 0)
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+@pytest.mark.parametrize("tokens", [2, 160])
+def test_large_and_infinite_logits(prec, tokens):
+    import torch
+    # logits of several hundreds: exp of them overflows, the result does not
+    p = Problem(prec, 64, tokens, 700, alpha=300.0, seed=13)
+    p.check_forward()
+    p.check_backward()
+    # logits of -inf take no part: a classifier row of -inf against positive hidden states
+    q = Problem(prec, 64, tokens, 700, seed=14, spread=0.0)
+    q.X.abs_()
+    q.label[q.label == 5] = 6
+    q.dlabel = torch.from_numpy(q.label.astype(np.int32)).cuda()
+    q.W[5] = -float("inf")
+    q.x64 = np.abs(q.x64)
+    q.w64[5] = -np.inf
+    q.check_forward()
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+@pytest.mark.parametrize("tokens", [4, 200])
+def test_same_bits_every_time_and_on_another_stream(prec, tokens):
+    import torch
+    p = Problem(prec, 264, tokens, 3000, seed=15, masked=0.2)
+    first = p.forward()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for stream in (None, side.cuda_stream):
+        again = p.forward(stream=stream)
+        assert all(np.array_equal(a, b) for a, b in zip(first, again))
+    a, b = p.check_backward(), p.check_backward()
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_nothing_to_do():
+    import torch
+    W = torch.randn(20, 8, device="cuda")
+    none = torch.empty(0, device="cuda")
+    labels = torch.empty(0, dtype=torch.int32, device="cuda")
+    loss, lse = blas.gpu_xent("s", 8, 0, 20, 1.0, W, 8, none, 8, labels)
+    assert loss.numel() == 0 and lse.numel() == 0
+    # no tokens: gW is beta times what it was, or zeros
+    gW = torch.ones(20, 8, device="cuda")
+    blas.gpu_xent_grad("s", 8, 0, 20, 1.0, W, 8, none, 8, labels, IGNORE, none, none, None, 0.5, gW, 8, none, 8)
+    assert (gW == 0.5).all()
+    gW.fill_(float("nan"))
+    blas.gpu_xent_grad("s", 8, 0, 20, 1.0, W, 8, none, 8, labels, IGNORE, none, none, None, 0.0, gW, 8, none, 8)
+    assert (gW == 0).all()
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+def test_training_step_captured_and_replayed(prec):
+    """Loss, gradients, their norm and clipping in one graph, replayed on new inputs with eager work in between, each
+    replay against the same calls made eagerly; then the chain against 64 bits."""
+    import torch
+    dt = {"s": torch.float32, "b": torch.bfloat16}[prec]
+    H, T, V = 320, 180, 2100
+    W = (torch.randn(V, H, device="cuda") * 2 / H ** 0.5).to(dt)
+    X = torch.randn(T, H, device="cuda").to(dt)
+    label = torch.randint(0, V, (T,), device="cuda", dtype=torch.int32)
+    gloss = torch.full((T,), 1.0, device="cuda")
+    gW, gX = torch.empty_like(W), torch.empty_like(X)
+    loss, lse, norm = torch.empty(T, device="cuda"), torch.empty(T, device="cuda"), torch.empty(1, device="cuda")
+    bias = torch.randn(777, device="cuda")
+    group = blas.TensorGroup([gW, gX])
+    out = blas.TensorGroup([torch.empty_like(gW), torch.empty_like(gX)])
+    work = torch.empty(max(blas.xent_worksize(prec, H, T, V), blas.xent_grad_worksize(prec, H, T, V)), dtype=torch.uint8,
+                       device="cuda")
+    nwork = torch.empty(blas.gnrm2_worksize(group), dtype=torch.uint8, device="cuda")
+
+    def step():
+        blas.gpu_xent(prec, H, T, V, 1.0, W, H, X, H, label, IGNORE, loss, lse, work=work)
+        blas.gpu_xent_grad(prec, H, T, V, 1.0, W, H, X, H, label, IGNORE, lse, gloss, None, 0.0, gW, H, gX, H, work=work)
+        blas.gpu_gnrm2(group, norm, work=nwork)
+        blas.gpu_gclip(group, norm, 0.5, out=out)
+
+    results = [loss, lse, gW, gX, norm] + out.tensors
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    for rep in range(4):
+        X.copy_(torch.randn(T, H, device="cuda"))
+        label.copy_(torch.randint(0, V, (T,), device="cuda"))
+        label[::rep + 2] = IGNORE
+        step()
+        torch.cuda.synchronize()
+        want = [x.clone() for x in results]
+        for x in results:
+            x.fill_(float("nan"))
+        (bias * 2).sum().item()
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(results, want):
+            assert torch.equal(a, b), rep
+    # the chain: what clipping returns has the norm asked for, and the norm is that of the gradients
+    n64 = sum(float(x.double().square().sum()) for x in (gW, gX)) ** 0.5
+    assert n64 > 0.5
+    assert abs(float(norm) - n64) <= 4 * 2.0 ** -24 * n64
+    half = xent_ref.half_step(prec)
+    for x, y in zip((gW, gX), out.tensors):
+        want = x.double() * (0.5 / n64)
+        assert ((y.double() - want).abs() <= (half + 8 * 2.0 ** -24) * want.abs() + 2.0 ** -133).all()
+    w64, x64 = W.double().cpu().numpy(), X.double().cpu().numpy()
+    lab = label.cpu().numpy()
+    wloss, wlse, blse, bloss = xent_ref.forward(w64, x64, lab, 1.0, IGNORE, prec)
+    assert (np.abs(loss.double().cpu().numpy() - wloss) <= bloss).all()
+    wW, wX, bW, bX = xent_ref.backward(w64, x64, lab, 1.0, IGNORE, lse.double().cpu().numpy(), np.ones(T), None, prec)
+    assert (np.abs(gW.double().cpu().numpy() - wW) <= bW).all()
+    assert (np.abs(gX.double().cpu().numpy() - wX) <= bX).all()
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+def test_two_calls_at_once(prec):
+    """Two streams, a workspace each: both get what a call by itself gets."""
+    import torch
+    ps = [Problem(prec, 256, t, 4000, seed=20 + t) for t in (9, 400)]
+    want = [p.forward() for p in ps]
+    streams = [torch.cuda.Stream() for _ in ps]
+    works = [p.work(blas.xent_worksize(prec, p.H, p.T, p.V)) for p in ps]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = [blas.gpu_xent(prec, p.H, p.T, p.V, p.alpha, p.W, p.ldW, p.X, p.ldX, p.dlabel, IGNORE, work=w,
+                             stream=s.cuda_stream) for p, s, w in zip(ps, streams, works)]
+        torch.cuda.synchronize()
+        for (l, e), (wl, we) in zip(got, want):
+            assert np.array_equal(l.double().cpu().numpy(), wl) and np.array_equal(e.double().cpu().numpy(), we)

@@ -1,0 +1,131 @@
+"""The cross entropy's formulas against differences, and what its entry points (and those of the group norm and
+clipping) refuse, without a device: every refusal is made on the host before anything is launched."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import xent_ref
+from ulmblas_amd import blas, lib
+
+BAD = 1
+
+
+def test_formula_against_differences():
+    rng = np.random.default_rng(1)
+    V, T, H, alpha = 23, 9, 7, 0.7
+    W, X = rng.standard_normal((V, H)), rng.standard_normal((T, H))
+    label = rng.integers(0, V, T)
+    label[[2, 5]] = [-100, V]
+    gloss, glse = rng.standard_normal(T), rng.standard_normal(T)
+
+    def value(W, X):
+        loss, lse, _, _ = xent_ref.forward(W, X, label, alpha, -100, "s")
+        return gloss @ loss + glse @ lse
+
+    _, lse, _, _ = xent_ref.forward(W, X, label, alpha, -100, "s")
+    gW, gX, _, _ = xent_ref.backward(W, X, label, alpha, -100, lse, gloss, glse, "s")
+    h = 1e-5
+    for name, A, g in (("W", W, gW), ("X", X, gX)):
+        for _ in range(5):
+            d = rng.standard_normal(A.shape)
+            up, down = (value(W + h * d, X), value(W - h * d, X)) if name == "W" else (value(W, X + h * d), value(W, X - h * d))
+            # h^2/6 times a third derivative of order |d|^3 ~ (VH)^1.5, and rounding 2^-53 |value| / h
+            assert abs((up - down) / (2 * h) - (g * d).sum()) < 1e-6, name
+
+
+P = C.c_void_p(4096)        # a pointer that nothing follows: the refusals come first
+
+
+def xent(p, hidden=8, tokens=4, vocab=10, ldW=8, ldX=8, W=P, X=P, label=P, loss=P, lse=P, work=P):
+    return getattr(lib.load(), f"ulmblas_gpu_{p}xent")(hidden, tokens, vocab, 1.0, W, ldW, X, ldX, label, -100, loss, lse,
+                                                       work, None)
+
+
+def grad(p, hidden=8, tokens=4, vocab=10, ldW=8, ldX=8, ldGW=8, ldGX=8, W=P, X=P, label=P, lse=P, gloss=P, gW=P, gX=P,
+         work=P):
+    return getattr(lib.load(), f"ulmblas_gpu_{p}xent_grad")(hidden, tokens, vocab, 1.0, W, ldW, X, ldX, label, -100, lse,
+                                                            gloss, None, 0.0, gW, ldGW, gX, ldGX, work, None)
+
+
+@pytest.mark.parametrize("p", ["s", "b"])
+def test_refusals_of_the_cross_entropy(p):
+    for kw in (dict(hidden=0, ldW=8), dict(hidden=-1), dict(hidden=(1 << 20) + 1, ldW=1 << 21, ldX=1 << 21), dict(tokens=-1),
+               dict(tokens=(1 << 28) + 1), dict(vocab=0), dict(vocab=(1 << 28) + 1), dict(ldW=7), dict(ldX=7), dict(W=None),
+               dict(X=None), dict(label=None), dict(loss=None), dict(lse=None), dict(work=None), dict(work=C.c_void_p(4104))):
+        assert xent(p, **kw) == BAD, kw
+        assert lib.load().ulmblas_gpu_last_error() != b""
+    for kw in (dict(hidden=0), dict(tokens=-1), dict(vocab=0), dict(ldW=7), dict(ldX=7), dict(ldGW=7), dict(ldGX=7),
+               dict(W=None), dict(X=None), dict(label=None), dict(lse=None), dict(gloss=None), dict(work=None),
+               dict(work=C.c_void_p(4104))):
+        assert grad(p, **kw) == BAD, kw
+    # nothing to do: no device is needed
+    assert xent(p, tokens=0, W=None, X=None, label=None, loss=None, lse=None, work=None) == 0
+    assert grad(p, gW=None, gX=None) == 0
+
+
+@pytest.mark.parametrize("p", ["s", "b"])
+def test_worksizes(p):
+    for bad in ((0, 1, 1), (1, -1, 1), (1, 1, 0), ((1 << 20) + 1, 1, 1)):
+        for f in (blas.xent_worksize, blas.xent_grad_worksize):
+            with pytest.raises(blas.GpuError):
+                f(p, *bad)
+    # the gradient keeps a piece of the vocabulary, never the logits: P, a packed piece of W and sums of gX
+    size = {"s": 4, "b": 2}[p]
+    big = blas.xent_grad_worksize(p, 4096, 1 << 16, 1 << 18)
+    assert big < (1 << 16) * (1 << 18) * size
+    # no tokens need what their bookkeeping takes, no more
+    assert blas.xent_worksize(p, 8, 0, 10) > 0 and blas.xent_grad_worksize(p, 8, 0, 10) > 0
+    # the largest sizes are counted in 64 bits
+    assert blas.xent_worksize(p, 1 << 20, 1 << 28, 1 << 28) > 1 << 40
+
+
+def group(count=2, type=b"sb", n=(4, 4), x=(4096, 4096), y=(4096, 4096), norm=P, work=P, largest=1.0, which="norm"):
+    L = lib.load()
+    lengths = (C.c_long * 2)(*n) if n else None
+    px = (C.c_void_p * 2)(*x) if x else None
+    py = (C.c_void_p * 2)(*y) if y else None
+    if which == "norm":
+        return L.ulmblas_gpu_gnrm2(count, type, lengths, px, norm, work, None)
+    return L.ulmblas_gpu_gclip(count, type, lengths, px, py, norm, largest, None)
+
+
+def test_refusals_of_the_group():
+    for which in ("norm", "clip"):
+        for kw in (dict(count=-1), dict(type=b"sd"), dict(type=None), dict(n=None), dict(x=None), dict(n=(-1, 4)),
+                   dict(n=((1 << 40) + 1, 4)), dict(x=(None, 4096)), dict(x=(4098, 4096)), dict(x=(4096, 4097)),
+                   dict(norm=None)):
+            assert group(which=which, **kw) == BAD, (which, kw)
+    assert group(work=None) == BAD and group(work=C.c_void_p(4100)) == BAD
+    for kw in (dict(largest=-1.0), dict(largest=float("nan")), dict(y=None), dict(y=(4098, 4096)), dict(y=(None, 4096))):
+        assert group(which="clip", **kw) == BAD, kw
+    assert group(which="clip", count=0, norm=None) == 0
+
+
+def test_wrappers_refuse_what_does_not_fit():
+    torch = pytest.importorskip("torch")
+    W, X = torch.zeros(10, 8), torch.zeros(4, 8)
+    label = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="not on a GPU"):
+        blas.gpu_xent("s", 8, 4, 10, 1.0, W, 8, X, 8, label)
+    with pytest.raises(ValueError, match="window"):
+        blas.gpu_xent("s", 8, 4, 11, 1.0, W, 8, X, 8, label)
+    with pytest.raises(ValueError, match="window"):
+        blas.gpu_xent("s", 8, 4, 10, 1.0, W, 8, X, 9, label)
+    with pytest.raises(TypeError, match="W must be"):
+        blas.gpu_xent("b", 8, 4, 10, 1.0, W, 8, X, 8, label)
+    with pytest.raises(TypeError, match="labels"):
+        blas.gpu_xent("s", 8, 4, 10, 1.0, W, 8, X, 8, label.long())
+    with pytest.raises(ValueError, match="labels"):
+        blas.gpu_xent("s", 8, 4, 10, 1.0, W, 8, X, 8, label[:3])
+    f = torch.zeros(4)
+    with pytest.raises(ValueError, match="gW"):
+        blas.gpu_xent_grad("s", 8, 4, 10, 1.0, W, 8, X, 8, label, -100, f, f, None, 0.0, torch.zeros(9, 8), 8, None, 8)
+    with pytest.raises(ValueError, match="lse"):
+        blas.gpu_xent_grad("s", 8, 4, 10, 1.0, W, 8, X, 8, label, -100, f[:2], f, None, 0.0, None, 8, None, 8)
+    with pytest.raises(TypeError, match="tensor 1"):
+        blas.TensorGroup([f, f.double()])
+    with pytest.raises(ValueError, match="contiguous"):
+        blas.TensorGroup([torch.zeros(4, 4).T])
+    with pytest.raises(ValueError, match="not on a GPU"):
+        blas.TensorGroup([f])

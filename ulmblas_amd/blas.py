@@ -277,7 +277,7 @@ def _dev_ptr(x):
     return C.c_void_p(x.data_ptr()) if x is not None else None
 
 
-_ELEMENT_BYTES = {"s": 4, "d": 8, "c": 8, "z": 16}
+_ELEMENT_BYTES = {"b": 2, "s": 4, "d": 8, "c": 8, "z": 16}
 
 
 def room(x):
@@ -438,8 +438,220 @@ def gpu_dlaswp(n, dA, ldA, k1, k2, dPiv, incPiv=1, stream=None):
     return dA
 
 
+# ---------------------------------------------------------------------------
+# softmax cross entropy of a classifier, its gradient, norm and clipping of the gradients
+# ---------------------------------------------------------------------------
+
+def _torch_type(prec):
+    import torch
+    return {"s": torch.float32, "b": torch.bfloat16}[prec]
+
+
+def _device_of(named):
+    """The one device that all tensors given live on."""
+    device = None
+    for name, x in named:
+        if x is None:
+            continue
+        if x.device.type != "cuda":
+            raise ValueError(f"{name} is not on a GPU")
+        if device is not None and x.device != device:
+            raise ValueError(f"{name} is on {x.device}, the operands before it on {device}")
+        device = x.device
+    return device
+
+
+class _On:
+    """The operands' device as the current one, with the stream to enqueue on (a raw
+    hipStream_t value, or None: torch's current stream of that device)."""
+
+    def __init__(self, device, stream):
+        import torch
+        self._guard, self._given, self._device = torch.cuda.device(device), stream, device
+
+    def __enter__(self):
+        import torch
+        self._guard.__enter__()
+        raw = torch.cuda.current_stream(self._device).cuda_stream if self._given is None else self._given
+        self.stream = C.c_void_p(raw)
+        return self
+
+    def __exit__(self, *exc):
+        return self._guard.__exit__(*exc)
+
+    def empty(self, n, dtype):
+        """A new tensor whose memory is not handed out again before the work on the stream is done."""
+        import torch
+        x = torch.empty(n, dtype=dtype, device=self._device)
+        if self._given is not None:
+            x.record_stream(torch.cuda.ExternalStream(self._given, device=self._device))
+        return x
+
+    def workspace(self, work, size):
+        """A caller's workspace, checked, or a new one."""
+        import torch
+        if work is None:
+            work = self.empty(size, torch.uint8)
+        elif room(work) < size:
+            raise ValueError(f"workspace of {room(work)} bytes, {size} are needed")
+        return work
+
+
+def _window(what, prec, x, rows, cols, ld):
+    """A typed rows x cols column-major window with leading dimension ld, as the kernels will read or write it."""
+    import torch
+    if x is None or cols <= 0:
+        return
+    if x.dtype != _torch_type(prec):
+        raise TypeError(f"{what} must be {_torch_type(prec)}")
+    _fits(what, prec, x, rows, cols, ld)
+
+
+def _vector(what, x, n, dtype):
+    if x is None:
+        return
+    if x.dtype != dtype:
+        raise TypeError(f"{what} must be {dtype}")
+    if not x.is_contiguous() or x.numel() < n:
+        raise ValueError(f"{what}: {n} consecutive elements are needed")
+
+
+def _worksize(name, hidden, tokens, vocab):
+    size = getattr(load(), name)(hidden, tokens, vocab)
+    if size == 0:
+        raise GpuError(f"{name}: invalid size")
+    return size
+
+
+def xent_worksize(prec, hidden, tokens, vocab):
+    """Bytes of workspace that gpu_xent needs."""
+    return _worksize(f"ulmblas_gpu_{prec}xent_worksize", hidden, tokens, vocab)
+
+
+def xent_grad_worksize(prec, hidden, tokens, vocab):
+    """Bytes of workspace that gpu_xent_grad needs."""
+    return _worksize(f"ulmblas_gpu_{prec}xent_grad_worksize", hidden, tokens, vocab)
+
+
+def gpu_xent(prec, hidden, tokens, vocab, alpha, dW, ldW, dX, ldX, dLabel, ignore=-100, dLoss=None, dLse=None, work=None,
+             stream=None):
+    """Cross entropy of every token's softmax over the vocabulary, without the logits (prec "s": float32, "b":
+    bfloat16 operands).  dW holds the classifier as a column-major hidden x vocab window (a torch [vocab, hidden]
+    matrix with row stride ldW), dX the hidden states likewise, dLabel int32 labels; tokens whose label is `ignore`
+    or no row of the classifier have loss and lse 0.  Returns (dLoss, dLse), float32, allocated unless given.
+    Asynchronous."""
+    import torch
+    _window("W", prec, dW, hidden, vocab, ldW)
+    _window("X", prec, dX, hidden, tokens, ldX)
+    _vector("labels", dLabel, tokens, torch.int32)
+    device = _device_of((("W", dW), ("X", dX), ("labels", dLabel), ("loss", dLoss), ("lse", dLse), ("work", work)))
+    size = xent_worksize(prec, hidden, tokens, vocab)
+    with _On(device, stream) as on:
+        dLoss = on.empty(tokens, torch.float32) if dLoss is None else dLoss
+        dLse = on.empty(tokens, torch.float32) if dLse is None else dLse
+        _vector("loss", dLoss, tokens, torch.float32)
+        _vector("lse", dLse, tokens, torch.float32)
+        work = on.workspace(work, size)
+        _status(getattr(load(), f"ulmblas_gpu_{prec}xent")(hidden, tokens, vocab, alpha, _dev_ptr(dW), ldW, _dev_ptr(dX),
+                                                           ldX, _dev_ptr(dLabel), ignore, _dev_ptr(dLoss),
+                                                           _dev_ptr(dLse), _dev_ptr(work), on.stream))
+    return dLoss, dLse
+
+
+def gpu_xent_grad(prec, hidden, tokens, vocab, alpha, dW, ldW, dX, ldX, dLabel, ignore, dLse, dGLoss, dGLse, beta, dGW,
+                  ldGW, dGX, ldGX, work=None, stream=None):
+    """Gradient of gpu_xent: dLse is its second result, dGLoss and dGLse (None: zero) the gradients of its results.
+    dGX (hidden x tokens) and dGW (hidden x vocab, alpha * X * P^T + beta * dGW) take the operands' type; None leaves
+    one out.  Returns (dGW, dGX).  Asynchronous."""
+    import torch
+    for name, x, cols, ld in (("W", dW, vocab, ldW), ("X", dX, tokens, ldX), ("gW", dGW, vocab, ldGW),
+                              ("gX", dGX, tokens, ldGX)):
+        _window(name, prec, x, hidden, cols, ld)
+    _vector("labels", dLabel, tokens, torch.int32)
+    for name, x in (("lse", dLse), ("gradient of loss", dGLoss), ("gradient of lse", dGLse)):
+        _vector(name, x, tokens, torch.float32)
+    device = _device_of((("W", dW), ("X", dX), ("labels", dLabel), ("lse", dLse), ("gradient of loss", dGLoss),
+                         ("gradient of lse", dGLse), ("gW", dGW), ("gX", dGX), ("work", work)))
+    size = xent_grad_worksize(prec, hidden, tokens, vocab)
+    with _On(device, stream) as on:
+        work = on.workspace(work, size)
+        _status(getattr(load(), f"ulmblas_gpu_{prec}xent_grad")(
+            hidden, tokens, vocab, alpha, _dev_ptr(dW), ldW, _dev_ptr(dX), ldX, _dev_ptr(dLabel), ignore,
+            _dev_ptr(dLse), _dev_ptr(dGLoss), _dev_ptr(dGLse), beta, _dev_ptr(dGW), ldGW, _dev_ptr(dGX), ldGX,
+            _dev_ptr(work), on.stream))
+    return dGW, dGX
+
+
+class TensorGroup:
+    """A list of float32 / bfloat16 tensors on one GPU as gpu_gnrm2 and gpu_gclip take it: the lists of addresses,
+    lengths and types are made once.  A program that passes the same tensors again keeps one; the group keeps its
+    tensors, and tensors whose memory is replaced need a new group."""
+
+    def __init__(self, tensors):
+        import torch
+        self.tensors = list(tensors)
+        kinds = {torch.float32: b"s", torch.bfloat16: b"b"}
+        for i, x in enumerate(self.tensors):
+            if x.dtype not in kinds:
+                raise TypeError(f"tensor {i} must be float32 or bfloat16")
+            if not x.is_contiguous():
+                raise ValueError(f"tensor {i} is not contiguous")
+        self.device = _device_of([(f"tensor {i}", x) for i, x in enumerate(self.tensors)])
+        n = len(self.tensors)
+        self.count = n
+        self.types = b"".join(kinds[x.dtype] for x in self.tensors)
+        self.lengths = (C.c_long * max(n, 1))(*[x.numel() for x in self.tensors])
+        self.pointers = (C.c_void_p * max(n, 1))(*[x.data_ptr() for x in self.tensors])
+
+
+def _as_group(tensors):
+    return tensors if isinstance(tensors, TensorGroup) else TensorGroup(tensors)
+
+
+def gnrm2_worksize(tensors):
+    """Bytes of workspace that gpu_gnrm2 needs for this TensorGroup or list."""
+    return load().ulmblas_gpu_gnrm2_worksize(tensors.count if isinstance(tensors, TensorGroup) else len(tensors))
+
+
+def gpu_gnrm2(tensors, dNorm=None, work=None, stream=None):
+    """Euclidean norm of a TensorGroup (or list of tensors) taken as one vector, into the float32 device tensor
+    dNorm (one element, allocated unless given), which is returned.  Asynchronous."""
+    import torch
+    g = _as_group(tensors)
+    device = _device_of((("tensors", g.tensors[0] if g.count else None), ("norm", dNorm), ("work", work)))
+    if device is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    with _On(device, stream) as on:
+        dNorm = on.empty(1, torch.float32) if dNorm is None else dNorm
+        _vector("norm", dNorm, 1, torch.float32)
+        work = on.workspace(work, gnrm2_worksize(g))
+        _status(load().ulmblas_gpu_gnrm2(g.count, g.types, g.lengths, g.pointers, _dev_ptr(dNorm), _dev_ptr(work),
+                                         on.stream))
+    return dNorm
+
+
+def gpu_gclip(tensors, dNorm, largest, out=None, stream=None):
+    """Multiplies a TensorGroup (or list of tensors) by min(1, largest / dNorm), in place or into the TensorGroup (or
+    list) `out` of the same lengths and types; returns the group that was written.  Asynchronous."""
+    import torch
+    g = _as_group(tensors)
+    o = g if out is None else _as_group(out)
+    if o.types != g.types or list(o.lengths) != list(g.lengths):
+        raise ValueError("out: lengths and types must be those of the tensors")
+    _vector("norm", dNorm, 1, torch.float32)
+    device = _device_of((("tensors", g.tensors[0] if g.count else None), ("out", o.tensors[0] if o.count else None),
+                         ("norm", dNorm)))
+    if g.count == 0:
+        return o
+    with _On(device, stream) as on:
+        _status(load().ulmblas_gpu_gclip(g.count, g.types, g.lengths, g.pointers, o.pointers, _dev_ptr(dNorm), largest,
+                                         on.stream))
+    return o
+
+
 TEST_NARROW_LOADS, TEST_LU_SPIN_LIMIT, TEST_SHARED_PIECES, TEST_SHARED_MUTE, TEST_SHARED_SPIN_LIMIT, TEST_FAIL_ALLOC, \
-    TEST_WHOLE_C, TEST_LU_SIMPLE_PANELS, TEST_TRSM_PARTS, TEST_HOST_HEAD, TEST_TRI_WAY = 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11
+    TEST_WHOLE_C, TEST_LU_SIMPLE_PANELS, TEST_TRSM_PARTS, TEST_HOST_HEAD, TEST_TRI_WAY, TEST_XENT_PIECE = \
+    1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12
 SHARED_PIECES_DEFAULT = 32      # the library's own setting of TEST_SHARED_PIECES
 
 

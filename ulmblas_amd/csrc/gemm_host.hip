@@ -1392,6 +1392,10 @@ int ulmblas_gpu_test_control(int what, long value)
         return ULMBLAS_GPU_OK;
     case ULMBLAS_GPU_TEST_TRSM_PARTS:
         return trsm_set_parts((int)value);
+    case ULMBLAS_GPU_TEST_XENT_PIECE:
+        if (value < 0 || value > 1 << 19) return ULMBLAS_GPU_BAD_ARGUMENT;
+        xent_set_piece_rows((int)value);
+        return ULMBLAS_GPU_OK;
     case ULMBLAS_GPU_TEST_HOST_HEAD:
         g_host_head.store((int)value);
         return ULMBLAS_GPU_OK;

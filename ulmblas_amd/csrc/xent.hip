@@ -1,0 +1,539 @@
+// Softmax cross entropy of a classifier over a large vocabulary, and its
+// gradient, straight from the hidden states and the classifier's weights:
+//
+//     z_tv = alpha sum_h x_th w_vh,   lse_t = log sum_v exp z_tv,
+//     loss_t = lse_t - z_t,label(t)
+//     P_tv = gloss_t (softmax(z_t)_v - [v = label(t)]) + glse_t softmax(z_t)_v
+//     gX = alpha P W,   gW = alpha P^T X + beta gW
+//
+// The logits are never kept.  The forward pass reduces them to one maximum and
+// one sum per token and tile of the vocabulary in the epilogue of the product
+// (product kernel: xent_kernel.hip.h); the backward pass computes them again,
+// a piece of the vocabulary at a time, and keeps P of one piece while the two
+// products that need it run.  Tokens without a target (their label is `ignore`
+// or no row of the classifier) are left out at the start: the rows of X that
+// count are gathered into a compact copy, every product runs over those rows
+// only, and what the other rows of X hold never reaches a result.
+//
+// Every sum is made in a fixed order: the same call gives the same bits.
+#include "internal.h"
+#include "xent_kernel.hip.h"
+
+#include <algorithm>
+#include <cstdio>
+
+using namespace ulmgpu;
+using namespace ulmgpu::xent;
+
+namespace ulmgpu {
+namespace {
+
+// ---------------------------------------------------------------------------
+// small kernels around the products
+// ---------------------------------------------------------------------------
+
+struct TokenArgs {
+    int tokens, vocab, ignore;
+    const int *label;
+    float *loss, *lse_out;              // forward: zeros for rows without a target (null: not wanted)
+    int *count, *rows, *label_c;        // rows that count, in order, and their labels
+    int *place;                         // backward: compact place of every row or -1
+    const float *lse, *gloss, *glse;    // backward: gathered and combined
+    float alpha;
+    float *lse_c, *both_c, *gloss_c;
+};
+
+// One workgroup: which rows have a target, in order.
+__global__ void __launch_bounds__(1024) token_kernel(TokenArgs g)
+{
+    __shared__ int wave_sum[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int done = 0;
+    for (int t0 = 0; t0 < g.tokens; t0 += 1024) {
+        const int t = t0 + (int)threadIdx.x;
+        int y = -1;
+        if (t < g.tokens) {
+            y = g.label[t];
+            if (y == g.ignore || y < 0 || y >= g.vocab) y = -1;
+        }
+        const unsigned long long votes = __builtin_amdgcn_ballot_w64(y >= 0);
+        if (lane == 0) wave_sum[wave] = __popcll(votes);
+        __syncthreads();
+        int before = done, all = done;
+        for (int w = 0; w < 16; ++w) {
+            before += w < wave ? wave_sum[w] : 0;
+            all += wave_sum[w];
+        }
+        const int c = before + __popcll(votes & ((1ull << lane) - 1));
+        if (y >= 0) {
+            g.rows[c] = t;
+            g.label_c[c] = y;
+            if (g.lse) {
+                const float gl = g.gloss[t];
+                g.lse_c[c] = g.lse[t];
+                g.gloss_c[c] = g.alpha * gl;
+                g.both_c[c] = g.alpha * (g.glse ? gl + g.glse[t] : gl);
+            }
+        } else if (t < g.tokens && g.loss) {
+            g.loss[t] = 0.0f;
+            g.lse_out[t] = 0.0f;
+        }
+        if (g.place && t < g.tokens) g.place[t] = y >= 0 ? c : -1;
+        done = all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *g.count = done;
+}
+
+// dst[c] <- src[rows ? rows[c] : c], padded with zeros to `width` elements.
+// One workgroup a row.
+template <typename T>
+__global__ void __launch_bounds__(256)
+gather_kernel(const T *__restrict__ src, int64_t ld, int cols, const int *rows, const int *count, T *__restrict__ dst,
+              int64_t width)
+{
+    const int c = blockIdx.x;
+    if (count && c >= *count) return;
+    const T *from = src + (rows ? rows[c] : c) * ld;
+    T *to = dst + c * width;
+    constexpr int V = 16 / sizeof(T);
+    if (((uintptr_t)from & 15) == 0) {
+        for (int64_t i = threadIdx.x * V; i < width; i += 256 * V) {
+            if (i + V <= cols) {
+                *reinterpret_cast<vint4 *>(to + i) = *reinterpret_cast<const vint4 *>(from + i);
+            } else {
+                for (int e = 0; e < V; ++e) to[i + e] = i + e < cols ? from[i + e] : T(0);
+            }
+        }
+    } else {
+        for (int64_t i = threadIdx.x; i < width; i += 256) to[i] = i < cols ? from[i] : T(0);
+    }
+}
+
+// lse and loss of every compact token from the statistics of the tiles: 64
+// tokens a workgroup, four threads each.
+template <typename T>
+__global__ void __launch_bounds__(256)
+loss_kernel(int tiles, const float2 *__restrict__ stats, int64_t ld, const float *__restrict__ target,
+            const int *__restrict__ rows, const int *__restrict__ count, float *loss, float *lse)
+{
+    __shared__ float2 part[4][64];
+    const int live = *count;
+    if ((int)blockIdx.x * 64 >= live) return;
+    const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
+    const int c = blockIdx.x * 64 + lane;
+    float top = -INFINITY, sum = 0.0f;
+    if (c < live) {
+        for (int i = slice; i < tiles; i += 4) {
+            const float2 s = stats[i * ld + c];
+            const float t = fmaxf(top, s.x);
+            const float from = t == -INFINITY ? 0.0f : t;
+            // an empty side has sum 0 and maximum -inf: exp(-inf) times 0
+            sum = sum * expf(top - from) + s.y * expf(s.x - from);
+            top = t;
+        }
+    }
+    part[slice][lane] = make_float2(top, sum);
+    __syncthreads();
+    if (slice == 0 && c < live) {
+        for (int k = 1; k < 4; ++k) top = fmaxf(top, part[k][lane].x);
+        const float from = top == -INFINITY ? 0.0f : top;
+        sum = 0.0f;
+        for (int k = 0; k < 4; ++k) sum += part[k][lane].y * expf(part[k][lane].x - from);
+        const float l = from + logf(sum);
+        const int t = rows[c];
+        lse[t] = l;
+        loss[t] = l - target[c];
+    }
+}
+
+// gX of every row: the sum over the splits in order, or zeros.
+template <typename T>
+__global__ void __launch_bounds__(256)
+gx_kernel(int hidden, const int *__restrict__ place, const float *__restrict__ part, int64_t ld, int64_t stride,
+          int splits, T *gx, int64_t ldgx)
+{
+    const int t = blockIdx.x, c = place[t];
+    T *to = gx + t * ldgx;
+    for (int h = threadIdx.x; h < hidden; h += 256) {
+        float v = 0.0f;
+        if (c >= 0)
+            for (int s = 0; s < splits; ++s) v += part[s * stride + c * ld + h];
+        to[h] = from_float<T>(v);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// sizes
+// ---------------------------------------------------------------------------
+
+constexpr int kMaxHidden = 1 << 20, kMaxRows = 1 << 28;
+
+// testing: at most this many vocabulary rows in a piece (0: by size)
+std::atomic<int> g_piece_rows{0};
+
+inline int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+
+// What the workspace holds and where; every part starts on 256 bytes.
+struct Layout {
+    int64_t tokens_p, hidden_p;         // rounded up: rows of compact copies, elements of their rows
+    int piece;                          // vocabulary rows at a time (gradient: of P; packing: of W)
+    int splits;                         // partial sums of gX
+    int64_t rows, label, place, lse, both, gloss, target, count, x, w, stats, p, part, bytes;
+};
+
+constexpr int64_t kPieceBytes = (int64_t)1 << 30;       // of P or of a packed copy of W, at the most
+
+template <typename T> Layout layout(int hidden, int tokens, int vocab, bool grad)
+{
+    Layout l{};
+    l.tokens_p = round_up(std::max(tokens, 1), 256);
+    l.hidden_p = round_up(hidden, kStep<T>);
+    const int64_t row = std::max(grad ? l.tokens_p : 0, l.hidden_p) * (int64_t)sizeof(T);
+    int64_t piece = std::max<int64_t>(kPieceBytes / row / 256 * 256, 256);
+    piece = std::min<int64_t>(piece, 1 << 19);
+    if (g_piece_rows.load() > 0) piece = std::min<int64_t>(piece, round_up(g_piece_rows.load(), 256));
+    l.piece = (int)std::min<int64_t>(piece, round_up(vocab, 256));
+    l.splits = 1;
+    if (grad) {
+        const int64_t tiles = (round_up(hidden, 128) / 128) * (l.tokens_p / 128);
+        l.splits = (int)std::min<int64_t>(8, std::max<int64_t>(1, 256 / tiles));
+        l.splits = (int)std::min<int64_t>(l.splits, std::max<int64_t>(1, l.piece / 1024));
+    }
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += round_up(bytes, 256);
+        return here;
+    };
+    l.count = take(4);
+    l.rows = take(4 * l.tokens_p);
+    l.label = take(4 * l.tokens_p);
+    l.target = take(4 * l.tokens_p);
+    if (grad) {
+        l.place = take(4 * l.tokens_p);
+        l.lse = take(4 * l.tokens_p);
+        l.both = take(4 * l.tokens_p);
+        l.gloss = take(4 * l.tokens_p);
+    }
+    l.x = take(l.tokens_p * l.hidden_p * (int64_t)sizeof(T));
+    l.w = take((int64_t)l.piece * l.hidden_p * (int64_t)sizeof(T));
+    if (!grad) {
+        l.stats = take((round_up(vocab, 256) / 128) * l.tokens_p * 8);
+    } else {
+        l.p = take(l.tokens_p * l.piece * (int64_t)sizeof(T));
+        l.part = take((int64_t)l.splits * l.tokens_p * l.hidden_p * 4);
+    }
+    l.bytes = at;
+    return l;
+}
+
+bool sizes_ok(int hidden, int tokens, int vocab)
+{
+    return hidden >= 1 && hidden <= kMaxHidden && tokens >= 0 && tokens <= kMaxRows && vocab >= 1 && vocab <= kMaxRows;
+}
+
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+
+template <typename T, Mode MODE, int BM, int BN, int WM, int WN>
+int launch_tile(const ProductArgs &g, hipStream_t stream)
+{
+    auto kernel = product_kernel<T, MODE, BM, BN, WM, WN>;
+    constexpr int lds = Product<T, MODE, BM, BN, WM, WN>::kLds;
+    // LDS above the 64 KiB default needs an explicit opt-in, once per kernel and device.
+    static std::atomic<unsigned> ready{0};
+    int dev = 0;
+    HIP_TRY(hipGetDevice(&dev));
+    if (dev >= 32 || !(ready.load() >> dev & 1)) {
+        HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                    lds));
+        if (dev < 32) ready.fetch_or(1u << dev);
+    }
+    const int64_t tiles = (int64_t)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN);
+    if (tiles > 0x7fffffff) {
+        g_last_error = "too many tiles for one launch";
+        return ULMBLAS_GPU_BAD_ARGUMENT;
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, MODE == GX ? (unsigned)g.splits : 1u), dim3(WM * WN * 64), lds,
+                       stream, g);
+    HIP_TRY(hipGetLastError());
+    return ULMBLAS_GPU_OK;
+}
+
+// The 256 x 256 tile where it fills most of the GPU's 256 CUs, else 128 x 128.
+bool large_tile(int M, int N) { return (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 200; }
+
+template <typename T, Mode MODE> int launch_product(const ProductArgs &g, hipStream_t stream)
+{
+    if (large_tile(g.M, g.N)) return launch_tile<T, MODE, 256, 256, 2, 4>(g, stream);
+    return launch_tile<T, MODE, 128, 128, 2, 2>(g, stream);
+}
+
+// Whether the product kernel can read W where it lies: rows on 16 bytes, no
+// row ending inside 16 bytes, and a tile's rows within 31 bits of each other.
+template <typename T> bool in_place(const T *W, int ldW, int hidden)
+{
+    return ((uintptr_t)W & 15) == 0 && ldW * sizeof(T) % 16 == 0 && hidden * sizeof(T) % 16 == 0 &&
+           (int64_t)ldW * (int64_t)sizeof(T) < (1 << 23);
+}
+
+template <typename T>
+int gather(const T *src, int64_t ld, int cols, const int *rows, const int *count, int n, T *dst, int64_t width,
+           hipStream_t stream)
+{
+    hipLaunchKernelGGL(gather_kernel<T>, dim3((unsigned)n), dim3(256), 0, stream, src, ld, cols, rows, count, dst,
+                       width);
+    HIP_TRY(hipGetLastError());
+    return ULMBLAS_GPU_OK;
+}
+
+int bad(const char *text)
+{
+    g_last_error = text;
+    return ULMBLAS_GPU_BAD_ARGUMENT;
+}
+
+template <typename T> T *part_of(void *work, int64_t at) { return reinterpret_cast<T *>(static_cast<char *>(work) + at); }
+
+template <typename T>
+int xent_device(int hidden, int tokens, int vocab, float alpha, const T *W, int ldW, const T *X, int ldX,
+                const int *label, int ignore, float *loss, float *lse, void *work, hipStream_t stream)
+{
+    if (!sizes_ok(hidden, tokens, vocab)) return bad("invalid size");
+    if (ldW < hidden || ldX < hidden) return bad("leading dimension smaller than hidden");
+    if (tokens == 0) return ULMBLAS_GPU_OK;
+    if (!W || !X || !label || !loss || !lse || !work) return bad("null operand or workspace");
+    if ((uintptr_t)work & 15) return bad("workspace not on 16 bytes");
+    const Layout l = layout<T>(hidden, tokens, vocab, false);
+    TokenArgs t{};
+    t.tokens = tokens;
+    t.vocab = vocab;
+    t.ignore = ignore;
+    t.label = label;
+    t.loss = loss;
+    t.lse_out = lse;
+    t.count = part_of<int>(work, l.count);
+    t.rows = part_of<int>(work, l.rows);
+    t.label_c = part_of<int>(work, l.label);
+    hipLaunchKernelGGL(token_kernel, dim3(1), dim3(1024), 0, stream, t);
+    HIP_TRY(hipGetLastError());
+    T *Xc = part_of<T>(work, l.x);
+    int rc = gather<T>(X, ldX, hidden, t.rows, t.count, tokens, Xc, l.hidden_p, stream);
+    if (rc) return rc;
+
+    ProductArgs g{};
+    g.B = Xc;
+    g.ldB = l.hidden_p * (int64_t)sizeof(T);
+    g.widthB = (int)l.hidden_p;
+    g.N = tokens;
+    g.K = hidden;
+    g.count = t.count;
+    g.alpha = alpha;
+    g.label = t.label_c;
+    g.ldStats = l.tokens_p;
+    g.target = part_of<float>(work, l.target);
+    const bool direct = in_place(W, ldW, hidden);
+    const int piece = direct ? vocab : l.piece;
+    int tiles = 0;
+    for (int v0 = 0; v0 < vocab; v0 += piece) {
+        g.M = std::min(piece, vocab - v0);
+        g.first = v0;
+        if (direct) {
+            g.A = W;
+            g.ldA = (int64_t)ldW * sizeof(T);
+            g.widthA = hidden;
+        } else {
+            T *Wp = part_of<T>(work, l.w);
+            if ((rc = gather<T>(W + (int64_t)v0 * ldW, ldW, hidden, nullptr, nullptr, g.M, Wp, l.hidden_p, stream)))
+                return rc;
+            g.A = Wp;
+            g.ldA = l.hidden_p * (int64_t)sizeof(T);
+            g.widthA = (int)l.hidden_p;
+        }
+        g.stats = part_of<float2>(work, l.stats) + (int64_t)tiles * l.tokens_p;
+        if ((rc = launch_product<T, STATS>(g, stream))) return rc;
+        const int bm = large_tile(g.M, g.N) ? 256 : 128;
+        tiles += (g.M + bm - 1) / bm;
+    }
+    hipLaunchKernelGGL(loss_kernel<T>, dim3((unsigned)((tokens + 63) / 64)), dim3(256), 0, stream, tiles,
+                       part_of<float2>(work, l.stats), l.tokens_p, g.target, t.rows, t.count, loss, lse);
+    HIP_TRY(hipGetLastError());
+    return ULMBLAS_GPU_OK;
+}
+
+template <typename T>
+int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W, int ldW, const T *X, int ldX,
+                     const int *label, int ignore, const float *lse, const float *gloss, const float *glse, float beta,
+                     T *gW, int ldGW, T *gX, int ldGX, void *work, hipStream_t stream)
+{
+    if (!sizes_ok(hidden, tokens, vocab)) return bad("invalid size");
+    if (ldW < hidden || ldX < hidden || (gW && ldGW < hidden) || (gX && ldGX < hidden))
+        return bad("leading dimension smaller than hidden");
+    if (!gW && !gX) return ULMBLAS_GPU_OK;
+    if (tokens > 0 && (!W || !X || !label || !lse || !gloss)) return bad("null operand");
+    if (!work) return bad("null workspace");
+    if ((uintptr_t)work & 15) return bad("workspace not on 16 bytes");
+    const Layout l = layout<T>(hidden, tokens, vocab, true);
+    TokenArgs t{};
+    t.tokens = tokens;
+    t.vocab = vocab;
+    t.ignore = ignore;
+    t.label = label;
+    t.count = part_of<int>(work, l.count);
+    t.rows = part_of<int>(work, l.rows);
+    t.label_c = part_of<int>(work, l.label);
+    t.place = part_of<int>(work, l.place);
+    t.lse = lse;
+    t.gloss = gloss;
+    t.glse = glse;
+    t.alpha = alpha;
+    t.lse_c = part_of<float>(work, l.lse);
+    t.both_c = part_of<float>(work, l.both);
+    t.gloss_c = part_of<float>(work, l.gloss);
+    hipLaunchKernelGGL(token_kernel, dim3(1), dim3(1024), 0, stream, t);
+    HIP_TRY(hipGetLastError());
+    T *Xc = part_of<T>(work, l.x), *P = part_of<T>(work, l.p);
+    int rc = ULMBLAS_GPU_OK;
+    if (tokens > 0 && (rc = gather<T>(X, ldX, hidden, t.rows, t.count, tokens, Xc, l.hidden_p, stream))) return rc;
+    const int64_t row_x = l.hidden_p * (int64_t)sizeof(T), row_p = (int64_t)l.piece * (int64_t)sizeof(T);
+    const bool direct = in_place(W, ldW, hidden);
+    for (int v0 = 0; v0 < vocab; v0 += l.piece) {
+        const int vn = std::min(l.piece, vocab - v0);
+        const T *Wv = W ? W + (int64_t)v0 * ldW : nullptr;
+        int64_t row_w = (int64_t)ldW * (int64_t)sizeof(T);
+        int width_w = hidden;
+        ProductArgs g{};
+        g.count = t.count;
+        g.alpha = alpha;
+        if (tokens > 0) {
+            if (!direct) {
+                T *Wp = part_of<T>(work, l.w);
+                if ((rc = gather<T>(Wv, ldW, hidden, nullptr, nullptr, vn, Wp, l.hidden_p, stream))) return rc;
+                Wv = Wp;
+                row_w = row_x;
+                width_w = (int)l.hidden_p;
+            }
+            g.A = Wv;
+            g.ldA = row_w;
+            g.widthA = width_w;
+            g.B = Xc;
+            g.ldB = row_x;
+            g.widthB = (int)l.hidden_p;
+            g.M = vn;
+            g.N = tokens;
+            g.K = hidden;
+            g.label = t.label_c;
+            g.first = v0;
+            g.lse = t.lse_c;
+            g.both = t.both_c;
+            g.gloss = t.gloss_c;
+            g.P = P;
+            g.ldP = l.piece;
+            if ((rc = launch_product<T, PROB>(g, stream))) return rc;
+        }
+        // the vocabulary of this piece, rounded to whole chunks: P holds zeros up to there
+        const int vn_p = (int)std::min<int64_t>(l.piece, round_up(vn, 16 / (int64_t)sizeof(T)));
+        if (gX && tokens > 0) {
+            g.A = Wv;
+            g.ldA = row_w;
+            g.widthA = width_w;
+            g.B = P;
+            g.ldB = row_p;
+            g.widthB = vn_p;
+            g.M = hidden;
+            g.N = tokens;
+            g.K = vn;
+            g.part = part_of<float>(work, l.part);
+            g.ldD = l.hidden_p;
+            g.splitStride = l.tokens_p * l.hidden_p;
+            g.splits = l.splits;
+            g.add = v0 > 0;
+            if ((rc = launch_product<T, GX>(g, stream))) return rc;
+        }
+        if (gW) {
+            g.A = Xc;
+            g.ldA = row_x;
+            g.widthA = (int)l.hidden_p;
+            g.B = P;
+            g.ldB = row_p;
+            g.widthB = vn_p;
+            g.M = hidden;
+            g.N = vn;
+            g.K = tokens;
+            g.out = gW + (int64_t)v0 * ldGW;
+            g.ldD = ldGW;
+            g.beta = beta;
+            g.vector_out = ((uintptr_t)g.out % (4 * sizeof(T))) == 0 && ldGW % 4 == 0;
+            if ((rc = launch_product<T, GW>(g, stream))) return rc;
+        }
+    }
+    if (gX && tokens > 0) {
+        hipLaunchKernelGGL(gx_kernel<T>, dim3((unsigned)tokens), dim3(256), 0, stream, hidden, t.place,
+                           part_of<float>(work, l.part), l.hidden_p, l.tokens_p * l.hidden_p, l.splits, gX,
+                           (int64_t)ldGX);
+        HIP_TRY(hipGetLastError());
+    }
+    return ULMBLAS_GPU_OK;
+}
+
+template <typename T> long worksize(int hidden, int tokens, int vocab, bool grad)
+{
+    if (!sizes_ok(hidden, tokens, vocab)) return 0;
+    return (long)layout<T>(hidden, tokens, vocab, grad).bytes;
+}
+
+}  // namespace
+
+void xent_set_piece_rows(int rows) { g_piece_rows.store(rows); }
+
+}  // namespace ulmgpu
+
+extern "C" {
+
+long ulmblas_gpu_sxent_worksize(int hidden, int tokens, int vocab) { return worksize<float>(hidden, tokens, vocab, false); }
+long ulmblas_gpu_bxent_worksize(int hidden, int tokens, int vocab) { return worksize<bf16_t>(hidden, tokens, vocab, false); }
+long ulmblas_gpu_sxent_grad_worksize(int hidden, int tokens, int vocab)
+{
+    return worksize<float>(hidden, tokens, vocab, true);
+}
+long ulmblas_gpu_bxent_grad_worksize(int hidden, int tokens, int vocab)
+{
+    return worksize<bf16_t>(hidden, tokens, vocab, true);
+}
+
+int ulmblas_gpu_sxent(int hidden, int tokens, int vocab, float alpha, const float *dW, int ldW, const float *dX, int ldX,
+                      const int *dLabel, int ignore, float *dLoss, float *dLse, void *work, void *stream)
+{
+    return xent_device<float>(hidden, tokens, vocab, alpha, dW, ldW, dX, ldX, dLabel, ignore, dLoss, dLse, work,
+                              static_cast<hipStream_t>(stream));
+}
+
+int ulmblas_gpu_bxent(int hidden, int tokens, int vocab, float alpha, const unsigned short *dW, int ldW,
+                      const unsigned short *dX, int ldX, const int *dLabel, int ignore, float *dLoss, float *dLse,
+                      void *work, void *stream)
+{
+    return xent_device<bf16_t>(hidden, tokens, vocab, alpha, dW, ldW, dX, ldX, dLabel, ignore, dLoss, dLse, work,
+                               static_cast<hipStream_t>(stream));
+}
+
+int ulmblas_gpu_sxent_grad(int hidden, int tokens, int vocab, float alpha, const float *dW, int ldW, const float *dX,
+                           int ldX, const int *dLabel, int ignore, const float *dLse, const float *dGLoss,
+                           const float *dGLse, float beta, float *dGW, int ldGW, float *dGX, int ldGX, void *work,
+                           void *stream)
+{
+    return xent_grad_device<float>(hidden, tokens, vocab, alpha, dW, ldW, dX, ldX, dLabel, ignore, dLse, dGLoss, dGLse,
+                                   beta, dGW, ldGW, dGX, ldGX, work, static_cast<hipStream_t>(stream));
+}
+
+int ulmblas_gpu_bxent_grad(int hidden, int tokens, int vocab, float alpha, const unsigned short *dW, int ldW,
+                           const unsigned short *dX, int ldX, const int *dLabel, int ignore, const float *dLse,
+                           const float *dGLoss, const float *dGLse, float beta, unsigned short *dGW, int ldGW,
+                           unsigned short *dGX, int ldGX, void *work, void *stream)
+{
+    return xent_grad_device<bf16_t>(hidden, tokens, vocab, alpha, dW, ldW, dX, ldX, dLabel, ignore, dLse, dGLoss, dGLse,
+                                    beta, dGW, ldGW, dGX, ldGX, work, static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"

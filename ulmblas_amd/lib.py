@@ -118,6 +118,23 @@ def load() -> C.CDLL:
     L.ulmblas_gpu_dgetrf_static.restype = i32
     L.ulmblas_gpu_dlaswp.argtypes = [i32, vp, i32, i32, i32, vp, i32, vp]
     L.ulmblas_gpu_dlaswp.restype = i32
+    # softmax cross entropy of a classifier and its gradient; bf16 operands (b) are device pointers like the others
+    for p_ in "sb":
+        for name in (f"ulmblas_gpu_{p_}xent_worksize", f"ulmblas_gpu_{p_}xent_grad_worksize"):
+            getattr(L, name).argtypes = [i32, i32, i32]
+            getattr(L, name).restype = C.c_long
+        getattr(L, f"ulmblas_gpu_{p_}xent").argtypes = [i32, i32, i32, flt, vp, i32, vp, i32, vp, i32, vp, vp, vp, vp]
+        getattr(L, f"ulmblas_gpu_{p_}xent").restype = i32
+        getattr(L, f"ulmblas_gpu_{p_}xent_grad").argtypes = [i32, i32, i32, flt, vp, i32, vp, i32, vp, i32, vp, vp, vp, flt,
+                                                             vp, i32, vp, i32, vp, vp]
+        getattr(L, f"ulmblas_gpu_{p_}xent_grad").restype = i32
+    # norm and clipping of a group of tensors
+    L.ulmblas_gpu_gnrm2_worksize.argtypes = [i32]
+    L.ulmblas_gpu_gnrm2_worksize.restype = C.c_long
+    L.ulmblas_gpu_gnrm2.argtypes = [i32, pc, C.POINTER(C.c_long), C.POINTER(vp), vp, vp, vp]
+    L.ulmblas_gpu_gnrm2.restype = i32
+    L.ulmblas_gpu_gclip.argtypes = [i32, pc, C.POINTER(C.c_long), C.POINTER(vp), C.POINTER(vp), vp, flt, vp]
+    L.ulmblas_gpu_gclip.restype = i32
     L.ulmblas_gpu_set_variant.argtypes = [i32, i32]
     L.ulmblas_gpu_set_variant.restype = i32
     L.ulmblas_gpu_test_control.argtypes = [i32, C.c_long]
