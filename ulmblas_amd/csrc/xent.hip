@@ -465,7 +465,7 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
             g.out = gW + (int64_t)v0 * ldGW;
             g.ldD = ldGW;
             g.beta = beta;
-            g.vector_out = ((uintptr_t)g.out % (4 * sizeof(T))) == 0 && ldGW % 4 == 0;
+            g.wide_out = (uintptr_t)g.out % 16 == 0 && ldGW * sizeof(T) % 16 == 0;
             if ((rc = launch_product<T, GW>(g, stream))) return rc;
         }
     }

@@ -88,7 +88,7 @@ struct ProductArgs {
     // GW
     void *out;
     float beta;
-    int vector_out;             // rows of out take 4 elements at a time
+    int wide_out;               // rows of out lie on 16 bytes
 };
 
 // Number of 16-byte chunks by which the chunks of row k of an operand that is
@@ -99,6 +99,11 @@ template <int CHUNKS> __device__ __forceinline__ int k_row_swizzle(int k)
     if constexpr (CHUNKS >= 16) return (k & 3) * 4;
     return ((k >> 1) & 1) * 4;
 }
+
+// The same for K-contiguous rows of 128 bytes: a read takes 16 rows at a time
+// from the 64 banks (256 bytes), so pairs of rows get the 8 chunks in turn
+// (rotating by the row itself costs every read twice its cycles).
+__device__ __forceinline__ int row_swizzle(int row) { return (row >> 1) & 7; }
 
 // Brings R rows (or columns) of one operand for one step into LDS.
 template <typename T, int R, bool KC, int WAVES>
@@ -113,7 +118,7 @@ struct Loader {
     int64_t left;               // bytes of the operand from there on
     int64_t ld;
     unsigned row_offset[kCalls];
-    unsigned k_chunk;           // KC: byte inside the step this lane fetches
+    unsigned k_chunk;           // KC: byte inside the step this lane fetches in even calls (odd ones: 64 bytes across)
     unsigned k_bytes;           // KC: bytes of a row that exist
 
     __device__ void init(const void *p, int64_t ld_, int row0, int rows, int width, int wave, int lane)
@@ -129,7 +134,7 @@ struct Loader {
             const int at = (wave * kCalls + c) * 64 + lane;
             const int row = at / kChunks, chunk = at % kChunks;
             if constexpr (KC) {
-                k_chunk = (unsigned)((chunk ^ (row & 7)) * 16);
+                if (c == 0) k_chunk = (unsigned)((chunk ^ row_swizzle(row)) * 16);
                 row_offset[c] = (unsigned)(row * ld);
             } else if constexpr (sizeof(T) == 2) {
                 row_offset[c] = (unsigned)(row * ld) + (unsigned)((chunk ^ k_row_swizzle<kChunks>(row)) * 16);
@@ -144,10 +149,12 @@ struct Loader {
     {
         uint64_t at = base;
         int64_t have = left;
-        unsigned k_offset = 0;
+        unsigned k_offset[2] = {0, 0};
         if constexpr (KC) {
-            k_offset = (unsigned)s * kStepBytes + k_chunk;
-            if (k_offset >= k_bytes) k_offset = kOutside;
+            k_offset[0] = (unsigned)s * kStepBytes + k_chunk;
+            k_offset[1] = k_offset[0] ^ 64u;
+            if (k_offset[0] >= k_bytes) k_offset[0] = kOutside;
+            if (k_offset[1] >= k_bytes) k_offset[1] = kOutside;
         } else {
             const int64_t skip = (int64_t)s * kStep<T> * ld;
             at += (uint64_t)skip;
@@ -162,7 +169,7 @@ struct Loader {
 #pragma unroll
         for (int c = 0; c < kCalls; ++c) {
             const unsigned lds = __builtin_amdgcn_readfirstlane(to + (unsigned)(wave * kCalls + c) * 1024u);
-            const unsigned off = row_offset[c] + k_offset;
+            const unsigned off = row_offset[c] + k_offset[c & 1];
             // writes LDS only: nothing here has a register for its result
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                          :
@@ -181,7 +188,7 @@ __device__ __forceinline__ vint4 fragment(lds_byte *tile, int r0, int kk, int la
 {
     if constexpr (KC) {
         const int r = r0 + (lane & 31), g = 2 * kk + (lane >> 5);
-        return *(__attribute__((address_space(3))) const vint4 *)(tile + r * kStepBytes + ((g ^ (r & 7)) << 4));
+        return *(__attribute__((address_space(3))) const vint4 *)(tile + r * kStepBytes + ((g ^ row_swizzle(r)) << 4));
     } else if constexpr (sizeof(T) == 2) {
         constexpr int kChunks = R / 8;
         typedef __attribute__((address_space(3))) vshort4 lds_short4;
@@ -229,12 +236,52 @@ template <typename T> __device__ __forceinline__ float exponential(float x)
     else return expf(x);
 }
 
+// Everything this wave has asked for has arrived, and every wave of the
+// workgroup says so.
+__device__ __forceinline__ void wait_and_meet()
+{
+    __builtin_amdgcn_s_waitcnt(0x0070);         // tells the compiler; the next line is what counts
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// Spreads the reads of the next quarter's fragments between the matrix
+// instructions of this one.
+template <int READS, int MFMA, int GROUPS, int I = 0> __device__ __forceinline__ void interleave()
+{
+    if constexpr (I < GROUPS) {
+        __builtin_amdgcn_sched_group_barrier(0x100, (READS * (I + 1)) / GROUPS - (READS * I) / GROUPS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, (MFMA * (I + 1)) / GROUPS - (MFMA * I) / GROUPS, 0);
+        interleave<READS, MFMA, GROUPS, I + 1>();
+    }
+}
+
+// Which tile of D workgroup `id` computes.  Workgroups go round the 8 XCDs;
+// each XCD takes a run of consecutive tiles, ordered in bands of 8 columns, so
+// that the 32 tiles its CUs work on at a time are 8 x 4 and share operands in
+// its L2.
+__device__ __forceinline__ bool tile_of(int id, int tilesM, int tilesN, int &tm, int &tn)
+{
+    const int tiles = tilesM * tilesN;
+    if (id >= tiles) return false;
+    const int per = tiles / 8, extra = tiles % 8, x = id % 8;
+    id = x * per + (x < extra ? x : extra) + id / 8;
+    const int band = id / (8 * tilesM), at = id % (8 * tilesM);
+    const int width = tilesN - band * 8 < 8 ? tilesN - band * 8 : 8;
+    tn = band * 8 + at % width;
+    tm = at / width;
+    return true;
+}
+
 template <typename T, Mode MODE, int BM, int BN, int WM, int WN>
 struct Product {
     static constexpr int kWaves = WM * WN;
     static constexpr int kThreads = kWaves * 64;
     static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;      // MFMA tiles of a wave
     static constexpr bool A_KC = MODE == STATS || MODE == PROB, B_KC = MODE != GW;
+    // a quarter of a step: LDS reads for its fragments (those staged along k take several), matrix instructions
+    static constexpr int kApart = sizeof(T) == 2 ? 2 : 4;
+    static constexpr int kReads = TM * (A_KC ? 1 : kApart) + TN * (B_KC ? 1 : kApart);
+    static constexpr int kMfma = TM * TN * (sizeof(T) == 2 ? 1 : 4);
     static constexpr int kStage = (BM + BN) * kStepBytes;
     static constexpr int kLds = 2 * kStage;
     using LoadA = Loader<T, BM, A_KC, kWaves>;
@@ -242,6 +289,42 @@ struct Product {
 
     static __device__ void run(const ProductArgs &g);
 };
+
+// The tile of a bf16 result on its way through LDS: rows of BM elements, the
+// 16-byte chunks of a row rotated by the row, so that neither the 8-byte writes
+// (32 rows at a time) nor the 16-byte reads (along a row) meet on a bank.
+template <int BM> __device__ __forceinline__ int staged_at(int row, int col)
+{
+    constexpr int kChunks = BM / 8;
+    return row * (BM * 2) + (((col >> 3) ^ (row & (kChunks - 1))) << 4) + (col & 7) * 2;
+}
+
+// Writes the staged tile out, whole rows at a time: rows x cols of it, 16 bytes
+// a lane where the rows lie on 16 bytes, else element by element.
+template <int BM, int THREADS>
+__device__ __forceinline__ void write_staged(const unsigned char *lds, bf16_t *to, int64_t ld, int rows, int cols,
+                                             bool wide)
+{
+    constexpr int kChunks = BM / 8;
+    if (wide) {
+        for (int i = threadIdx.x; i < rows * kChunks; i += THREADS) {
+            const int row = i / kChunks, col = i % kChunks * 8;
+            if (col >= cols) continue;
+            const vint4 v = *reinterpret_cast<const vint4 *>(lds + staged_at<BM>(row, col));
+            bf16_t *p = to + row * ld + col;
+            if (col + 8 <= cols) {
+                *reinterpret_cast<vint4 *>(p) = v;
+            } else {
+                for (int e = 0; e < cols - col; ++e) p[e] = reinterpret_cast<const bf16_t *>(&v)[e];
+            }
+        }
+    } else {
+        for (int i = threadIdx.x; i < rows * BM; i += THREADS) {
+            const int row = i / BM, col = i % BM;
+            if (col < cols) to[row * ld + col] = *reinterpret_cast<const bf16_t *>(lds + staged_at<BM>(row, col));
+        }
+    }
+}
 
 template <typename T, Mode MODE, int BM, int BN, int WM, int WN>
 __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
@@ -253,19 +336,12 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
 
-    // Workgroups go round the 8 XCDs; each XCD takes a run of consecutive tiles.
-    const int tilesM = (g.M + BM - 1) / BM, tilesN = (g.N + BN - 1) / BN;
-    const int tiles = tilesM * tilesN;
-    int id = blockIdx.x;
-    {
-        const int per = tiles / 8, extra = tiles % 8, x = id % 8;
-        id = x * per + (x < extra ? x : extra) + id / 8;
-    }
-    const int tm = id % tilesM, tn = id / tilesM;
-    const int m0 = tm * BM, n0 = tn * BN;
+    // Columns past the tokens that count have no tile.
     const int live = __builtin_amdgcn_readfirstlane(*g.count);
     const int boundN = MODE == GW ? g.N : (live < g.N ? live : g.N);
-    if (n0 >= boundN) return;
+    int tm, tn;
+    if (!tile_of((int)blockIdx.x, (g.M + BM - 1) / BM, (boundN + BN - 1) / BN, tm, tn)) return;
+    const int m0 = tm * BM, n0 = tn * BN;
     const int K = MODE == GW ? (live < g.K ? live : g.K) : g.K;
     int s0 = 0, s1 = (K + kStep<T> - 1) / kStep<T>;
     if constexpr (MODE == GX) {
@@ -288,37 +364,61 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
+    // Two halves of LDS, a step each; within a step four quarters, whose fragments are read one quarter ahead.
+    // The step changes before the last quarter is multiplied: its fragments are in registers by then, so the
+    // half just read can be refilled (for the step after next) and the matrix cores have work while the waves
+    // meet and the next step's first fragments come out of LDS.
     if (s0 < s1) {
         la.fetch(s0, lds0, wave);
         lb.fetch(s0, lds0 + BM * kStepBytes, wave);
-    }
-    for (int s = s0; s < s1; ++s) {
-        // this step's tile is in LDS, and nobody reads the other half any more
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const unsigned now = ((s - s0) & 1) * kStage, next = kStage - now;
-        if (s + 1 < s1) {
-            la.fetch(s + 1, lds0 + next, wave);
-            lb.fetch(s + 1, lds0 + next + BM * kStepBytes, wave);
-        }
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            vint4 a[TM], b[TN];
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-                a[i] = fragment<T, BM, A_KC>(lds + now, (wm * TM + i) * 32, kk, lane);
+        vint4 a[2][TM], b[2][TN];
+        auto read = [&](int buf, unsigned half, int kk) {
 #pragma unroll
             for (int j = 0; j < TN; ++j)
-                b[j] = fragment<T, BN, B_KC>(lds + now + BM * kStepBytes, (wn * TN + j) * 32, kk, lane);
+                b[buf][j] = fragment<T, BN, B_KC>(lds + half + BM * kStepBytes, (wn * TN + j) * 32, kk, lane);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+                a[buf][i] = fragment<T, BM, A_KC>(lds + half, (wm * TM + i) * 32, kk, lane);
+        };
+        auto quarter = [&](int buf) {
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = multiply<T>(a[i], b[j], acc[i][j]);
+                for (int j = 0; j < TN; ++j) acc[i][j] = multiply<T>(a[buf][i], b[buf][j], acc[i][j]);
+            interleave<kReads, kMfma, (kReads < kMfma ? kReads : kMfma)>();
+        };
+        wait_and_meet();
+        unsigned now = 0;
+        if (s0 + 1 < s1) {
+            la.fetch(s0 + 1, lds0 + kStage, wave);
+            lb.fetch(s0 + 1, lds0 + kStage + BM * kStepBytes, wave);
         }
+        read(0, now, 0);
+        auto first_three = [&] {
+#pragma unroll
+            for (int kk = 0; kk < 3; ++kk) {
+                read((kk + 1) & 1, now, kk + 1);
+                quarter(kk & 1);
+            }
+        };
+        for (int s = s0; s + 1 < s1; ++s) {
+            first_three();
+            wait_and_meet();
+            if (s + 2 < s1) {
+                la.fetch(s + 2, lds0 + now, wave);
+                lb.fetch(s + 2, lds0 + now + BM * kStepBytes, wave);
+            }
+            now = kStage - now;
+            read(0, now, 0);
+            quarter(1);
+        }
+        first_three();
+        quarter(1);
     }
 
     const int mw = m0 + wm * TM * 32 + (lane >> 5) * 4, nw = n0 + wn * TN * 32 + (lane & 31);
     if constexpr (MODE == STATS) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        wait_and_meet();
         float2 *red = reinterpret_cast<float2 *>(lds_raw);      // [wm][column]
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
@@ -367,6 +467,7 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
         // Rounded to the operands' type, since the two products that follow run on it: each element is off by
         // at most half a step (bf16: 2^-9 of itself), and the sums over tokens or vocabulary average that out.
         T *P = static_cast<T *>(g.P);
+        if constexpr (sizeof(T) == 2) wait_and_meet();
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
             const int n = nw + j * 32;
@@ -385,13 +486,18 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
                         if (m + r == want) p -= gloss;
                         v[r] = from_float<T>(m + r < g.M ? p : 0.0f);
                     }
-                    T *to = P + (int64_t)n * g.ldP + m;
                     if constexpr (sizeof(T) == 2) {
-                        *reinterpret_cast<vint2 *>(to) = *reinterpret_cast<vint2 *>(v);
+                        *reinterpret_cast<vint2 *>(lds_raw + staged_at<BM>(n - n0, m - m0)) =
+                            *reinterpret_cast<vint2 *>(v);
                     } else {
-                        *reinterpret_cast<vint4 *>(to) = *reinterpret_cast<vint4 *>(v);
+                        *reinterpret_cast<vint4 *>(P + (int64_t)n * g.ldP + m) = *reinterpret_cast<vint4 *>(v);
                     }
                 }
+        }
+        if constexpr (sizeof(T) == 2) {
+            __syncthreads();
+            write_staged<BM, kThreads>(lds_raw, P + (int64_t)n0 * g.ldP + m0, g.ldP,
+                                       boundN - n0 < BN ? boundN - n0 : BN, BM, true);
         }
     } else if constexpr (MODE == GX) {
         float *part = g.part + (int64_t)blockIdx.y * g.splitStride;
@@ -416,6 +522,7 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
         }
     } else {
         T *out = static_cast<T *>(g.out);
+        if constexpr (sizeof(T) == 2) wait_and_meet();
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
             const int n = nw + j * 32;
@@ -426,28 +533,30 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
                 for (int q = 0; q < 4; ++q) {
                     const int m = mw + i * 32 + q * 8;
                     T *to = out + (int64_t)n * g.ldD + m;
+                    float x[4];
                     T v[4];
-                    if (g.vector_out && m + 4 <= g.M) {
-                        using V = std::conditional_t<sizeof(T) == 2, vint2, vint4>;
-                        V old{};
-                        if (g.beta != 0.0f) old = *reinterpret_cast<const V *>(to);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            float x = acc[i][j][4 * q + r];
-                            if (g.beta != 0.0f) x += g.beta * to_float(reinterpret_cast<const T *>(&old)[r]);
-                            v[r] = from_float<T>(x);
-                        }
-                        *reinterpret_cast<V *>(to) = *reinterpret_cast<V *>(v);
+                    for (int r = 0; r < 4; ++r) {
+                        x[r] = acc[i][j][4 * q + r];
+                        if (g.beta != 0.0f && m + r < g.M) x[r] += g.beta * to_float(to[r]);
+                        v[r] = from_float<T>(x[r]);
+                    }
+                    if constexpr (sizeof(T) == 2) {
+                        *reinterpret_cast<vint2 *>(lds_raw + staged_at<BM>(n - n0, m - m0)) =
+                            *reinterpret_cast<vint2 *>(v);
+                    } else if (g.wide_out && m + 4 <= g.M) {
+                        *reinterpret_cast<vint4 *>(to) = *reinterpret_cast<vint4 *>(v);
                     } else {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            if (m + r >= g.M) continue;
-                            float x = acc[i][j][4 * q + r];
-                            if (g.beta != 0.0f) x += g.beta * to_float(to[r]);
-                            to[r] = from_float<T>(x);
-                        }
+                        for (int r = 0; r < 4; ++r)
+                            if (m + r < g.M) to[r] = v[r];
                     }
                 }
+        }
+        if constexpr (sizeof(T) == 2) {
+            __syncthreads();
+            write_staged<BM, kThreads>(lds_raw, out + (int64_t)n0 * g.ldD + m0, g.ldD, g.N - n0 < BN ? g.N - n0 : BN,
+                                       g.M - m0 < BM ? g.M - m0 : BM, g.wide_out);
         }
     }
 }
