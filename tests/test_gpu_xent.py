@@ -153,6 +153,37 @@ def test_rows_without_a_target(prec, tokens, masked):
 
 
 @pytest.mark.parametrize("prec", ["s", "b"])
+@pytest.mark.parametrize("labels", [[3], [127, 128], [0, 255, 256, 899]])
+def test_many_tokens_of_one_label(prec, labels):
+    import torch
+    p = Problem(prec, 328, 700, 900, seed=31, masked=0.1)
+    has = xent_ref.valid(p.label, p.V, IGNORE)
+    p.label[has] = np.resize(np.array(labels), int(has.sum()))
+    p.dlabel = torch.from_numpy(p.label.astype(np.int32)).cuda()
+    p.check_forward()
+    p.check_backward(beta=0.5)
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+def test_confident_and_equal_gradients(prec):
+    """Every token's loss has the same gradient, and some labels take nearly all of the softmax: what rounding takes from
+    their elements is the same for all tokens and would not average out."""
+    p = Problem(prec, 256, 300, 1000, seed=32, spread=4.0)
+    p.gloss[:] = 1.0 / 300
+    p.check_forward()
+    p.check_backward(glse=False)
+
+
+@pytest.mark.parametrize("alpha", [-0.8, 0.0])
+@pytest.mark.parametrize("tokens", [3, 140])
+def test_scale_of_the_logits_may_be_negative_or_zero(alpha, tokens):
+    for prec in "sb":
+        p = Problem(prec, 96, tokens, 777, seed=33, alpha=alpha)
+        p.check_forward()
+        p.check_backward()
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
 def test_ignore_may_be_a_row_of_the_classifier(prec):
     import torch
     p = Problem(prec, 64, 40, 50, seed=9)

@@ -9,7 +9,7 @@ the operands' type (fp32 2^-24, bf16 2^-8), the bounds are sums of these parts:
   and waves, one for every tile of 128 vocabulary rows; each exponential is off by at most 4 u of itself (2 u of the
   function, 2 u of its rounded argument near the maximum, where it counts);
 * P = both * exp(z - lse) - gloss is off by (2 max|dz| + 2 u |lse| + 8 u) of both * exp, by 4 u of gloss, and by v of
-  itself where it is rounded;  z - lse is formed in fp32, hence the 2 u |z - lse| <= 2 u (|z| + |lse|) that is added;
+  itself where it is rounded (not at the label, where what the rounding took is added in fp32);  z - lse is formed in fp32, hence the 2 u |z - lse| <= 2 u (|z| + |lse|) that is added;
 * exp, P and the operands of the matrix cores may lose what lies below the smallest normal number, 2^-126 in both types:
   up to 2^-126 of each P, since a value under it may be rounded on coarser steps or to zero;
 * the products sum tokens or vocabulary in fp32: (K + 8) u of the sum of absolute products, K their length;
@@ -69,7 +69,7 @@ def backward(W, X, label, alpha, ignore, lse, gloss, glse, prec, beta=0.0, gW0=N
         size = (np.abs(gloss[t]) + (0.0 if glse is None else np.abs(glse[t])))[:, None]
         dP = abs(alpha) * (size * p * (2 * dz + 2 * U * (np.abs(z) + 2 * np.abs(lse[t][:, None])) + 12 * U)
                            + 4 * U * np.abs(gloss[t])[:, None] * hot)
-        dP += v * (np.abs(P) + dP) + 2.0 ** -126
+        dP += np.where(hot == 1.0, 4 * U, v) * (np.abs(P) + dP) + 2.0 ** -126
         A = np.abs(P) + dP
         gX[t] = P @ w
         bX[t] = dP @ np.abs(w) + (V + 8) * U * (A @ np.abs(w))

@@ -85,6 +85,47 @@ __global__ void __launch_bounds__(1024) token_kernel(TokenArgs g)
     if (threadIdx.x == 0) *g.count = done;
 }
 
+// The tokens in the order of the group of 128 vocabulary rows that their label
+// is in, and within a group in their own order: one workgroup a group (the last
+// one only says where the list ends), which counts the labels below its group
+// and then puts its own behind them.
+__global__ void __launch_bounds__(256)
+bucket_kernel(const int *__restrict__ count, const int *__restrict__ label, int2 *member, int *rank, int *bucket)
+{
+    __shared__ int wave_sum[4];
+    const int live = *count, mine = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int below = 0, here = 0;
+    for (int c = threadIdx.x; c < live; c += 256) {
+        const int b = label[c] / 128;
+        below += b < mine;
+        here += b == mine;
+    }
+    for (int d = 32; d; d >>= 1) below += __shfl_xor(below, d);
+    if (lane == 0) wave_sum[wave] = below;
+    const int any = __syncthreads_or(here);
+    int at = wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
+    if (threadIdx.x == 0) bucket[mine] = at;
+    if (!any) return;
+    for (int c0 = 0; c0 < live; c0 += 256) {
+        const int c = c0 + threadIdx.x;
+        const bool is = c < live && label[c] / 128 == mine;
+        const unsigned long long votes = __builtin_amdgcn_ballot_w64(is);
+        __syncthreads();
+        if (lane == 0) wave_sum[wave] = __popcll(votes);
+        __syncthreads();
+        int before = at;
+        for (int w = 0; w < 4; ++w) {
+            before += w < wave ? wave_sum[w] : 0;
+            at += wave_sum[w];
+        }
+        if (is) {
+            const int place = before + __popcll(votes & ((1ull << lane) - 1));
+            member[place] = make_int2(c, label[c]);
+            rank[c] = place;
+        }
+    }
+}
+
 // dst[c] <- src[rows ? rows[c] : c], padded with zeros to `width` elements.
 // One workgroup a row.
 template <typename T>
@@ -147,16 +188,20 @@ loss_kernel(int tiles, const float2 *__restrict__ stats, int64_t ld, const float
     }
 }
 
-// gX of every row: the sum over the splits in order, or zeros.
+// gX of every row: the sum over the splits in order (bf16: and what rounding
+// took from P at the label), or zeros.
 template <typename T>
 __global__ void __launch_bounds__(256)
 gx_kernel(int hidden, const int *__restrict__ place, const float *__restrict__ part, int64_t ld, int64_t stride,
-          int splits, T *gx, int64_t ldgx)
+          int splits, const float *__restrict__ delta, const int *__restrict__ rank, const int *__restrict__ label, const T *__restrict__ W, int64_t ldw,
+          T *gx, int64_t ldgx)
 {
     const int t = blockIdx.x, c = place[t];
     T *to = gx + t * ldgx;
+    const float d = sizeof(T) == 2 && c >= 0 ? delta[rank[c]] : 0.0f;
+    const T *w = c >= 0 ? W + label[c] * ldw : W;
     for (int h = threadIdx.x; h < hidden; h += 256) {
-        float v = 0.0f;
+        float v = sizeof(T) == 2 && c >= 0 ? d * to_float(w[h]) : 0.0f;
         if (c >= 0)
             for (int s = 0; s < splits; ++s) v += part[s * stride + c * ld + h];
         to[h] = from_float<T>(v);
@@ -179,7 +224,7 @@ struct Layout {
     int64_t tokens_p, hidden_p;         // rounded up: rows of compact copies, elements of their rows
     int piece;                          // vocabulary rows at a time (gradient: of P; packing: of W)
     int splits;                         // partial sums of gX
-    int64_t rows, label, place, lse, both, gloss, target, count, x, w, stats, p, part, bytes;
+    int64_t rows, label, place, lse, both, gloss, delta, target, bucket, member, rank, count, x, w, stats, p, part, bytes;
 };
 
 constexpr int64_t kPieceBytes = (int64_t)1 << 30;       // of P or of a packed copy of W, at the most
@@ -215,6 +260,10 @@ template <typename T> Layout layout(int hidden, int tokens, int vocab, bool grad
         l.lse = take(4 * l.tokens_p);
         l.both = take(4 * l.tokens_p);
         l.gloss = take(4 * l.tokens_p);
+        l.delta = take(4 * l.tokens_p);
+        l.member = take(8 * l.tokens_p);
+        l.rank = take(4 * l.tokens_p);
+        l.bucket = take(4 * (round_up(vocab, 128) / 128 + 1));
     }
     l.x = take(l.tokens_p * l.hidden_p * (int64_t)sizeof(T));
     l.w = take((int64_t)l.piece * l.hidden_p * (int64_t)sizeof(T));
@@ -397,7 +446,17 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
     T *Xc = part_of<T>(work, l.x), *P = part_of<T>(work, l.p);
     int rc = ULMBLAS_GPU_OK;
     if (tokens > 0 && (rc = gather<T>(X, ldX, hidden, t.rows, t.count, tokens, Xc, l.hidden_p, stream))) return rc;
-    const int64_t row_x = l.hidden_p * (int64_t)sizeof(T), row_p = (int64_t)l.piece * (int64_t)sizeof(T);
+    float *delta = part_of<float>(work, l.delta);
+    int2 *member = part_of<int2>(work, l.member);
+    int *rank = part_of<int>(work, l.rank), *bucket = part_of<int>(work, l.bucket);
+    if (sizeof(T) == 2) {
+        hipLaunchKernelGGL(bucket_kernel, dim3((unsigned)(round_up(vocab, 128) / 128 + 1)), dim3(256), 0, stream, t.count,
+                           t.label_c, member, rank, bucket);
+        HIP_TRY(hipGetLastError());
+    }
+    // P: rows of blocks; all of them
+    const int64_t row_x = l.hidden_p * (int64_t)sizeof(T), row_p = (int64_t)l.piece / kStep<T> * kBlockBytes;
+    const int blocks_p = (int)(l.tokens_p / kBlockTokens * (l.piece / kStep<T>));
     const bool direct = in_place(W, ldW, hidden);
     for (int v0 = 0; v0 < vocab; v0 += l.piece) {
         const int vn = std::min(l.piece, vocab - v0);
@@ -430,18 +489,18 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
             g.both = t.both_c;
             g.gloss = t.gloss_c;
             g.P = P;
-            g.ldP = l.piece;
+            g.ldP = row_p;
+            g.rank = rank;
+            g.delta = delta;
             if ((rc = launch_product<T, PROB>(g, stream))) return rc;
         }
-        // the vocabulary of this piece, rounded to whole chunks: P holds zeros up to there
-        const int vn_p = (int)std::min<int64_t>(l.piece, round_up(vn, 16 / (int64_t)sizeof(T)));
         if (gX && tokens > 0) {
             g.A = Wv;
             g.ldA = row_w;
             g.widthA = width_w;
             g.B = P;
             g.ldB = row_p;
-            g.widthB = vn_p;
+            g.widthB = blocks_p;
             g.M = hidden;
             g.N = tokens;
             g.K = vn;
@@ -458,10 +517,14 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
             g.widthA = (int)l.hidden_p;
             g.B = P;
             g.ldB = row_p;
-            g.widthB = vn_p;
+            g.widthB = blocks_p;
             g.M = hidden;
             g.N = vn;
             g.K = tokens;
+            g.first = v0;
+            g.delta = delta;
+            g.bucket = bucket;
+            g.member = member;
             g.out = gW + (int64_t)v0 * ldGW;
             g.ldD = ldGW;
             g.beta = beta;
@@ -471,7 +534,8 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
     }
     if (gX && tokens > 0) {
         hipLaunchKernelGGL(gx_kernel<T>, dim3((unsigned)tokens), dim3(256), 0, stream, hidden, t.place,
-                           part_of<float>(work, l.part), l.hidden_p, l.tokens_p * l.hidden_p, l.splits, gX,
+                           part_of<float>(work, l.part), l.hidden_p, l.tokens_p * l.hidden_p, l.splits, delta, rank,
+                           t.label_c, W, (int64_t)ldW, gX,
                            (int64_t)ldGX);
         HIP_TRY(hipGetLastError());
     }

@@ -1,21 +1,21 @@
 // The product kernel behind the softmax cross entropy (xent.hip).
 //
 // One workgroup computes a BM x BN tile of D = A * B^T with accumulators in
-// fp32, for bf16 (v_mfma_f32_32x32x16_bf16) or fp32 (v_mfma_f32_32x32x2_f32)
+// fp32, for bf16 (v_mfma_f32_16x16x32_bf16) or fp32 (v_mfma_f32_16x16x4_f32)
 // operands, and hands it to one of four epilogues:
 //
 //   STATS  D = logits (A = W: vocabulary rows, B = X: tokens): the running
 //          maximum and sum of the softmax over the tile's BM vocabulary rows,
 //          per token, and the logit of the label; the logits stay in registers
 //   PROB   the same product again, turned into the gradient with respect to
-//          the logits, which is stored for the two products below
+//          the logits, P, which is stored for the two products below
 //   GX     gX^T += W^T * P  (A = W, read along k; B = P)
 //   GW     gW^T  = X^T * P  (A = X, B = P, both read along k)
 //
-// The column of D that a lane of the 32 x 32 MFMA holds is one token (STATS,
-// PROB), and its registers run along the vocabulary: the softmax reduces
-// inside the lane first, with one exchange between the two halves of the wave
-// and one through LDS between the waves of a column.
+// The column of D that a lane of the MFMA holds is one token (STATS, PROB), and
+// its registers run along the vocabulary: the softmax reduces inside the lane
+// first, with two exchanges between the lanes of a column and one through LDS
+// between the waves of a column.
 //
 // Operands come in two layouts.  "K-contiguous" rows (W and X in the logits,
 // P in GX) are staged as rows of 128 bytes; operands whose k runs across rows
@@ -25,6 +25,18 @@
 // kinds travel from global memory straight into LDS, 16 bytes a lane; what
 // lies outside the operand is fetched out of the buffer's range, which stores
 // zeros.
+//
+// P is kept in blocks of 256 tokens by 128 bytes of vocabulary, 32 KB without
+// a gap, so that what GX takes of it in one step is one such block and what GW
+// takes is 8 KB at a time (rows of P 128 KB apart: 3.53 ms for the GX product
+// 4096 x 8192 x 65536, in blocks 3.32 ms).
+//
+// Measured on bf16 tiles of 256 x 256, K = 65536 (GX) and 4096 (STATS): the
+// matrix cores are busy 70 % of the time at the 1.8 - 2.1 GHz that the power
+// limit leaves.  With the fetches left out the same loop runs 25 % faster,
+// with all of them served by L2 10 % faster; more steps in flight (up to 2) do
+// not help.  16 x 16 MFMAs run at a higher clock than 32 x 32 ones (they read
+// and write half the accumulators per product): STATS 1.90 -> 1.81 ms.
 #ifndef ULMBLAS_XENT_KERNEL_HIP_H
 #define ULMBLAS_XENT_KERNEL_HIP_H 1
 
@@ -62,25 +74,35 @@ constexpr int kStepBytes = 128;         // what one step of the k loop takes of 
 template <typename T> constexpr int kStep = kStepBytes / (int)sizeof(T);
 constexpr unsigned kOutside = 0x80000000u;      // an offset past every buffer's range
 
+// blocks of P
+constexpr int kBlockTokens = 256, kBlockBytes = kBlockTokens * kStepBytes;
+
 enum Mode { STATS, PROB, GX, GW };
+
+// How an operand lies in memory: rows along k; rows across k; P, taken along
+// the vocabulary (its k) or across the tokens (its k).
+enum Lie { ALONG, ACROSS, P_ALONG, P_ACROSS };
+constexpr bool k_contiguous(Lie lie) { return lie == ALONG || lie == P_ALONG; }
 
 struct ProductArgs {
     const void *A, *B;
-    int64_t ldA, ldB;           // bytes from row to row
+    int64_t ldA, ldB;           // bytes from row to row (P: from one row of blocks to the next)
     int M, N, K;                // rows of D, columns of D, length of the inner products
-    int widthA, widthB;         // elements of a row of A / B that exist (K-contiguous: K may end inside a step)
+    int widthA, widthB;         // elements of a row of A / B that exist (P: blocks in all)
     const int *count;           // tokens with a target: bounds N (STATS, PROB, GX) or K (GW)
     float alpha;
-    // STATS
     const int *label;           // per token (compact order)
+    int first;                  // first vocabulary row of A (STATS, PROB) or column of D (GW)
+    // STATS
     float2 *stats;              // [tile of the vocabulary][token]: maximum, sum of exp(z - maximum)
     int64_t ldStats;
     float *target;              // the label's logit
-    int first;                  // first vocabulary row of A
     // PROB
     const float *lse, *both, *gloss;    // per token; both = gloss + glse, each times alpha
     void *P;
-    int64_t ldP;                // elements
+    int64_t ldP;                // bytes from one row of blocks to the next
+    const int *rank;            // per token: its place in `member`
+    float *delta;               // per place there: what rounding took from P at the label (PROB writes, GW reads)
     // GX: partial sums of the splits, each [token][ldD]
     float *part;
     int64_t ldD, splitStride;
@@ -89,15 +111,17 @@ struct ProductArgs {
     void *out;
     float beta;
     int wide_out;               // rows of out lie on 16 bytes
+    const int *bucket;          // first place of each group of 128 vocabulary rows
+    const int2 *member;         // tokens (compact) in the order of their label's group, and their labels
 };
 
-// Number of 16-byte chunks by which the chunks of row k of an operand that is
-// staged along k are rotated (exclusive or), so that the four rows that one
-// transposing read takes do not fall on the same banks.
-template <int CHUNKS> __device__ __forceinline__ int k_row_swizzle(int k)
+// Chunks of 16 bytes of an operand staged across k are rotated (exclusive or) by
+// its row, so that the rows that one read takes (four groups of lanes, four rows
+// each in bf16) spread over the 64 banks.
+template <typename T, int CHUNKS> __device__ __forceinline__ int across_swizzle(int k)
 {
-    if constexpr (CHUNKS >= 16) return (k & 3) * 4;
-    return ((k >> 1) & 1) * 4;
+    if constexpr (sizeof(T) == 2) return ((k & 3) * 4 + ((k >> 3) & 1) * 2) & (CHUNKS - 1);
+    return ((k >> 2) & 3) * 4;
 }
 
 // The same for K-contiguous rows of 128 bytes: a read takes 16 rows at a time
@@ -106,26 +130,35 @@ template <int CHUNKS> __device__ __forceinline__ int k_row_swizzle(int k)
 __device__ __forceinline__ int row_swizzle(int row) { return (row >> 1) & 7; }
 
 // Brings R rows (or columns) of one operand for one step into LDS.
-template <typename T, int R, bool KC, int WAVES>
+template <typename T, int R, Lie LIE, int WAVES>
 struct Loader {
     static constexpr int kBytes = R * kStepBytes;
     static constexpr int kCalls = kBytes / 1024 / WAVES;        // 1024 bytes a wave and call
-    static constexpr int kRowBytes = KC ? kStepBytes : R * (int)sizeof(T);
+    static constexpr bool kAlong = k_contiguous(LIE);
+    static constexpr int kRowBytes = kAlong ? kStepBytes : R * (int)sizeof(T);
     static constexpr int kChunks = kRowBytes / 16;
+    static constexpr int kStepsPerBlock = kBlockTokens / kStep<T>;
     static_assert(kCalls * WAVES * 1024 == kBytes, "the waves share the tile evenly");
 
     uint64_t base;              // of the tile
     int64_t left;               // bytes of the operand from there on
     int64_t ld;
     unsigned row_offset[kCalls];
-    unsigned k_chunk;           // KC: byte inside the step this lane fetches in even calls (odd ones: 64 bytes across)
-    unsigned k_bytes;           // KC: bytes of a row that exist
+    unsigned k_chunk;           // ALONG: byte inside the step this lane fetches in even calls (odd ones: 64 across)
+    unsigned k_bytes;           // ALONG: bytes of a row that exist
 
     __device__ void init(const void *p, int64_t ld_, int row0, int rows, int width, int wave, int lane)
     {
         ld = ld_;
-        const int64_t total = rows > 0 ? (int64_t)(rows - 1) * ld + (int64_t)width * (int64_t)sizeof(T) : 0;
-        const int64_t skip = KC ? (int64_t)row0 * ld : (int64_t)row0 * (int64_t)sizeof(T);
+        int64_t total, skip;
+        if constexpr (LIE == ALONG || LIE == ACROSS) {
+            total = rows > 0 ? (int64_t)(rows - 1) * ld + (int64_t)width * (int64_t)sizeof(T) : 0;
+            skip = LIE == ALONG ? (int64_t)row0 * ld : (int64_t)row0 * (int64_t)sizeof(T);
+        } else {
+            total = (int64_t)width * kBlockBytes;
+            skip = LIE == P_ALONG ? (row0 / kBlockTokens) * ld + (row0 % kBlockTokens) * kStepBytes
+                                  : (int64_t)(row0 / kStep<T>) * kBlockBytes;
+        }
         base = (uint64_t)p + (uint64_t)skip;
         left = total - skip;
         k_bytes = (unsigned)width * (unsigned)sizeof(T);
@@ -133,106 +166,128 @@ struct Loader {
         for (int c = 0; c < kCalls; ++c) {
             const int at = (wave * kCalls + c) * 64 + lane;
             const int row = at / kChunks, chunk = at % kChunks;
-            if constexpr (KC) {
+            if constexpr (LIE == ALONG) {
                 if (c == 0) k_chunk = (unsigned)((chunk ^ row_swizzle(row)) * 16);
                 row_offset[c] = (unsigned)(row * ld);
-            } else if constexpr (sizeof(T) == 2) {
-                row_offset[c] = (unsigned)(row * ld) + (unsigned)((chunk ^ k_row_swizzle<kChunks>(row)) * 16);
+            } else if constexpr (LIE == P_ALONG) {
+                row_offset[c] = (unsigned)(row * kStepBytes + (chunk ^ row_swizzle(row)) * 16);
             } else {
-                row_offset[c] = (unsigned)(row * ld) + (unsigned)(chunk * 16);
+                const int from = chunk ^ across_swizzle<T, kChunks>(row);
+                row_offset[c] = LIE == ACROSS ? (unsigned)(row * ld) + (unsigned)(from * 16)
+                                              : (unsigned)(from / 8 * kBlockBytes + row * kStepBytes + from % 8 * 16);
             }
         }
     }
 
-    // step s of the k loop into the LDS bytes from `to` on
-    __device__ __forceinline__ void fetch(int s, unsigned to, int wave) const
+    // step s of the k loop: the buffer and the offsets its calls use
+    __device__ __forceinline__ void aim(int s, vint4 &rsrc, unsigned (&k_offset)[2]) const
     {
-        uint64_t at = base;
-        int64_t have = left;
-        unsigned k_offset[2] = {0, 0};
-        if constexpr (KC) {
+        int64_t skip = 0;
+        k_offset[0] = k_offset[1] = 0;
+        if constexpr (LIE == ALONG) {
             k_offset[0] = (unsigned)s * kStepBytes + k_chunk;
             k_offset[1] = k_offset[0] ^ 64u;
             if (k_offset[0] >= k_bytes) k_offset[0] = kOutside;
             if (k_offset[1] >= k_bytes) k_offset[1] = kOutside;
+        } else if constexpr (LIE == ACROSS) {
+            skip = (int64_t)s * kStep<T> * ld;
+        } else if constexpr (LIE == P_ALONG) {
+            skip = (int64_t)s * kBlockBytes;
         } else {
-            const int64_t skip = (int64_t)s * kStep<T> * ld;
-            at += (uint64_t)skip;
-            have -= skip;
+            skip = (int64_t)(s / kStepsPerBlock) * ld + s % kStepsPerBlock * (kStep<T> * kStepBytes);
         }
+        const uint64_t at = base + (uint64_t)skip;
+        int64_t have = left - skip;
         have = have < 0 ? 0 : (have > 0x7fffffff ? 0x7fffffff : have);
-        vint4 rsrc;
         rsrc[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)at);
         rsrc[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32) & 0xffff);
         rsrc[2] = __builtin_amdgcn_readfirstlane((int)have);
         rsrc[3] = 0x00020000;
-#pragma unroll
-        for (int c = 0; c < kCalls; ++c) {
-            const unsigned lds = __builtin_amdgcn_readfirstlane(to + (unsigned)(wave * kCalls + c) * 1024u);
-            const unsigned off = row_offset[c] + k_offset[c & 1];
-            // writes LDS only: nothing here has a register for its result
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                         :
-                         : "s"(lds), "v"(off), "s"(rsrc)
-                         : "memory");
-        }
+    }
+
+    // call c of a step into the tile at LDS byte `to`; writes LDS only: nothing here has a register for its result
+    __device__ __forceinline__ void call(int c, vint4 rsrc, const unsigned (&k_offset)[2], unsigned to, int wave) const
+    {
+        const unsigned lds = __builtin_amdgcn_readfirstlane(to + (unsigned)(wave * kCalls + c) * 1024u);
+        const unsigned off = row_offset[c] + k_offset[c & 1];
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                     :
+                     : "s"(lds), "v"(off), "s"(rsrc)
+                     : "memory");
     }
 };
 
 typedef __attribute__((address_space(3))) const unsigned char lds_byte;
 
-// 16 bytes of operand for one lane: bf16, 8 consecutive k of one row (column);
-// fp32, 4 consecutive k.  kk: quarter of the step.
-template <typename T, int R, bool KC>
-__device__ __forceinline__ vint4 fragment(lds_byte *tile, int r0, int kk, int lane)
-{
-    if constexpr (KC) {
-        const int r = r0 + (lane & 31), g = 2 * kk + (lane >> 5);
-        return *(__attribute__((address_space(3))) const vint4 *)(tile + r * kStepBytes + ((g ^ row_swizzle(r)) << 4));
-    } else if constexpr (sizeof(T) == 2) {
-        constexpr int kChunks = R / 8;
-        typedef __attribute__((address_space(3))) vshort4 lds_short4;
-        const int m = r0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-        vshort8 v;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int k = 16 * kk + 8 * (lane >> 5) + 4 * j + ((lane >> 2) & 3);
-            const int at = k * (R * 2) + (((m >> 3) ^ k_row_swizzle<kChunks>(k)) << 4) + (m & 7) * 2;
-            const vshort4 h = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(tile + at));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 * j + i] = h[i];
+// Fragments: 16 bytes of operand for one lane (bf16: 8 consecutive k of one row
+// or column; fp32: 4).  base() is the byte in the tile from which this lane
+// reads the first fragment of its wave, read() fragment x (16 rows on) of half
+// kk of the step.  The rotations of the chunks touch bits of the address that x
+// and kk own alone, so a fragment is an exclusive or and a constant away.
+template <typename T, int R, bool KC> struct Fragment {
+    static __device__ __forceinline__ unsigned base(int first, int lane)
+    {
+        if constexpr (KC) {
+            const int r = first + (lane & 15);
+            return (unsigned)(r * kStepBytes + (((lane >> 4) ^ row_swizzle(r)) << 4));
+        } else if constexpr (sizeof(T) == 2) {
+            const int m = first + (lane & 3) * 4, k = 8 * (lane >> 4) + ((lane >> 2) & 3);
+            return (unsigned)(k * (R * 2) + (((m >> 3) ^ across_swizzle<T, R / 8>(k)) << 4) + (m & 7) * 2);
+        } else {
+            const int m = first + (lane & 15), k = 4 * (lane >> 4);
+            return (unsigned)(k * (R * 4) + (((m >> 2) ^ across_swizzle<T, R / 4>(k)) << 4) + (m & 3) * 4);
         }
-        return __builtin_bit_cast(vint4, v);
-    } else {
-        vint4 v;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int k = 8 * kk + 4 * (lane >> 5) + j;
-            v[j] = *(__attribute__((address_space(3))) const int *)(tile + (k * R + r0 + (lane & 31)) * 4);
-        }
-        return v;
     }
-}
+    static __device__ __forceinline__ vint4 read(lds_byte *tile, unsigned base, int x, int kk)
+    {
+        if constexpr (KC) {
+            return *(__attribute__((address_space(3))) const vint4 *)(tile + (base ^ (unsigned)(kk << 6)) + x * (16 * kStepBytes));
+        } else if constexpr (sizeof(T) == 2) {
+            typedef __attribute__((address_space(3))) vshort4 lds_short4;
+            vshort8 v;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const vshort4 h = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_short4 *)(tile + (base ^ (unsigned)(x << 5)) + (32 * kk + 4 * j) * (R * 2)));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[4 * j + i] = h[i];
+            }
+            return __builtin_bit_cast(vint4, v);
+        } else {
+            vint4 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[j] = *(__attribute__((address_space(3))) const int *)(tile + (base ^ (unsigned)(x << 6)) +
+                                                                       (16 * kk + j) * (R * 4));
+            return v;
+        }
+    }
+};
 
 template <typename T>
-__device__ __forceinline__ vfloat16 multiply(vint4 a, vint4 b, vfloat16 c)
+__device__ __forceinline__ vfloat4 multiply(vint4 a, vint4 b, vfloat4 c)
 {
     if constexpr (sizeof(T) == 2) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vbf8, a), __builtin_bit_cast(vbf8, b), c, 0,
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vbf8, a), __builtin_bit_cast(vbf8, b), c, 0,
                                                        0, 0);
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            c = __builtin_amdgcn_mfma_f32_32x32x2f32(__int_as_float(a[j]), __int_as_float(b[j]), c, 0, 0, 0);
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__int_as_float(a[j]), __int_as_float(b[j]), c, 0, 0, 0);
         return c;
     }
 }
 
-// exp(x): bf16 results take the hardware's exponential (its argument is
-// rounded at 2^-24 of |x| log2 e, far below bf16), fp32 the library's.
+// exp(scale * x): for bf16 the hardware's exponential with log2 e in the scale
+// (its argument is rounded at 2^-24 of itself, far below bf16), for fp32 the
+// library's.
+template <typename T> __device__ __forceinline__ float scale_of(float alpha)
+{
+    return sizeof(T) == 2 ? alpha * 1.4426950408889634f : alpha;
+}
 template <typename T> __device__ __forceinline__ float exponential(float x)
 {
-    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(x * 1.4426950408889634f);
+    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(x);
     else return expf(x);
 }
 
@@ -242,17 +297,6 @@ __device__ __forceinline__ void wait_and_meet()
 {
     __builtin_amdgcn_s_waitcnt(0x0070);         // tells the compiler; the next line is what counts
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
-
-// Spreads the reads of the next quarter's fragments between the matrix
-// instructions of this one.
-template <int READS, int MFMA, int GROUPS, int I = 0> __device__ __forceinline__ void interleave()
-{
-    if constexpr (I < GROUPS) {
-        __builtin_amdgcn_sched_group_barrier(0x100, (READS * (I + 1)) / GROUPS - (READS * I) / GROUPS, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, (MFMA * (I + 1)) / GROUPS - (MFMA * I) / GROUPS, 0);
-        interleave<READS, MFMA, GROUPS, I + 1>();
-    }
 }
 
 // Which tile of D workgroup `id` computes.  Workgroups go round the 8 XCDs;
@@ -276,16 +320,14 @@ template <typename T, Mode MODE, int BM, int BN, int WM, int WN>
 struct Product {
     static constexpr int kWaves = WM * WN;
     static constexpr int kThreads = kWaves * 64;
-    static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;      // MFMA tiles of a wave
-    static constexpr bool A_KC = MODE == STATS || MODE == PROB, B_KC = MODE != GW;
-    // a quarter of a step: LDS reads for its fragments (those staged along k take several), matrix instructions
-    static constexpr int kApart = sizeof(T) == 2 ? 2 : 4;
-    static constexpr int kReads = TM * (A_KC ? 1 : kApart) + TN * (B_KC ? 1 : kApart);
-    static constexpr int kMfma = TM * TN * (sizeof(T) == 2 ? 1 : 4);
+    static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;      // MFMA tiles of a wave
+    static constexpr Lie LIE_A = MODE == STATS || MODE == PROB ? ALONG : ACROSS;
+    static constexpr Lie LIE_B = MODE == GX ? P_ALONG : MODE == GW ? P_ACROSS : ALONG;
+    static constexpr bool A_KC = k_contiguous(LIE_A), B_KC = k_contiguous(LIE_B);
     static constexpr int kStage = (BM + BN) * kStepBytes;
     static constexpr int kLds = 2 * kStage;
-    using LoadA = Loader<T, BM, A_KC, kWaves>;
-    using LoadB = Loader<T, BN, B_KC, kWaves>;
+    using LoadA = Loader<T, BM, LIE_A, kWaves>;
+    using LoadB = Loader<T, BN, LIE_B, kWaves>;
 
     static __device__ void run(const ProductArgs &g);
 };
@@ -310,18 +352,82 @@ __device__ __forceinline__ void write_staged(const unsigned char *lds, bf16_t *t
         for (int i = threadIdx.x; i < rows * kChunks; i += THREADS) {
             const int row = i / kChunks, col = i % kChunks * 8;
             if (col >= cols) continue;
-            const vint4 v = *reinterpret_cast<const vint4 *>(lds + staged_at<BM>(row, col));
+            const unsigned char *v = lds + staged_at<BM>(row, col);
             bf16_t *p = to + row * ld + col;
             if (col + 8 <= cols) {
-                *reinterpret_cast<vint4 *>(p) = v;
+                *reinterpret_cast<vint4 *>(p) = *reinterpret_cast<const vint4 *>(v);
             } else {
-                for (int e = 0; e < cols - col; ++e) p[e] = reinterpret_cast<const bf16_t *>(&v)[e];
+                for (int e = 0; e < cols - col; ++e) p[e] = reinterpret_cast<const bf16_t *>(v)[e];
             }
         }
     } else {
         for (int i = threadIdx.x; i < rows * BM; i += THREADS) {
             const int row = i / BM, col = i % BM;
             if (col < cols) to[row * ld + col] = *reinterpret_cast<const bf16_t *>(lds + staged_at<BM>(row, col));
+        }
+    }
+}
+
+// Where element (token n, vocabulary row m) of P lies.
+template <typename T> __device__ __forceinline__ int64_t p_byte(int n, int m, int64_t ld)
+{
+    return n / kBlockTokens * ld + (int64_t)(m / kStep<T>) * kBlockBytes + n % kBlockTokens * kStepBytes +
+           m % kStep<T> * (int)sizeof(T);
+}
+
+// The tile of gW^T starts from what rounding took from P at the labels: for
+// every token whose label is one of the tile's columns, delta times its x.  The
+// tokens are found through the groups of 128 vocabulary rows they are sorted by,
+// 64 of them at a time, and those of this wave's columns are taken in pairs, so
+// that their rows of x are on the way together; all of it runs while the first
+// step is fetched.
+template <typename T, int BM, int BN, int WM, int WN>
+__device__ __forceinline__ void add_label_remainders(const ProductArgs &g, int m0, int n0, int wm, int wn, int lane,
+                                                     vfloat4 (&acc)[BM / WM / 16][BN / WN / 16])
+{
+    constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
+    const int v0 = g.first + n0, v1 = v0 + BN < g.first + g.N ? v0 + BN : g.first + g.N;
+    const int from = __builtin_amdgcn_readfirstlane(g.bucket[v0 / 128]);
+    const int to = __builtin_amdgcn_readfirstlane(g.bucket[(v1 + 127) / 128]);
+    for (int e0 = from; e0 < to; e0 += 64) {
+        const int e = e0 + lane < to ? e0 + lane : to - 1;
+        const int2 member = g.member[e];
+        const float delta = g.delta[e];
+        const int column = member.y - v0;
+        unsigned long long mine = __builtin_amdgcn_ballot_w64(e0 + lane < to && column / (TN * 16) == wn);
+        while (mine) {
+            int n[2];
+            float d[2];
+            vint2 x[2][TM];
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const int at = mine ? __builtin_ctzll(mine) : 0;
+                n[p] = __builtin_amdgcn_readlane(column, at) % (TN * 16);
+                const float dp = mine ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(delta), at)) : 0.0f;
+                d[p] = (lane & 15) == n[p] % 16 ? dp : 0.0f;
+                const T *row = reinterpret_cast<const T *>(static_cast<const char *>(g.A) +
+                                                           __builtin_amdgcn_readlane(member.x, at) * g.ldA);
+#pragma unroll
+                for (int i = 0; i < TM; ++i) {
+                    const int m = m0 + (wm * TM + i) * 16 + (lane >> 4) * 4;
+                    x[p][i] = vint2{0, 0};
+                    if (m < g.widthA) x[p][i] = *reinterpret_cast<const vint2 *>(row + m);
+                }
+                mine &= mine - 1;
+            }
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+#pragma unroll
+                for (int i = 0; i < TM; ++i) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float f = d[p] * to_float((bf16_t)((unsigned)x[p][i][r >> 1] >> 16 * (r & 1)));
+#pragma unroll
+                        for (int j = 0; j < TN; ++j) acc[i][j][r] += n[p] / 16 == j ? f : 0.0f;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);      // keeps the unpacked values of one row of tiles at a time
+                }
+            }
         }
     }
 }
@@ -352,103 +458,166 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
 
     LoadA la;
     LoadB lb;
-    // K-contiguous: rows of D's side, of `width` elements; else rows of k
+    // ALONG: rows of D's side, of `width` elements; ACROSS: rows of k
     la.init(g.A, g.ldA, m0, A_KC ? g.M : K, g.widthA, wave, lane);
-    lb.init(g.B, g.ldB, n0, B_KC ? g.N : K, g.widthB, wave, lane);
+    lb.init(g.B, g.ldB, n0, B_KC ? boundN : K, g.widthB, wave, lane);
 
-    vfloat16 acc[TM][TN];
+    vfloat4 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+            for (int r = 0; r < 4; ++r) acc[i][j][r] = 0.0f;
 
-    // Two halves of LDS, a step each; within a step four quarters, whose fragments are read one quarter ahead.
-    // The step changes before the last quarter is multiplied: its fragments are in registers by then, so the
-    // half just read can be refilled (for the step after next) and the matrix cores have work while the waves
-    // meet and the next step's first fragments come out of LDS.
+    // Two halves of LDS, a step each; a step is two halves of k, and the TM rows
+    // of MFMA tiles of one half are a group each.  The fragment of A is read
+    // three groups ahead into a ring of four, those of B for one half of k while
+    // the other half is multiplied.  The step changes three groups before its
+    // end: all its fragments are in registers by then, so the half just read can
+    // be refilled for the step after next, and the matrix cores have work while
+    // the waves meet and the next step's first fragments come out of LDS.
     if (s0 < s1) {
-        la.fetch(s0, lds0, wave);
-        lb.fetch(s0, lds0 + BM * kStepBytes, wave);
-        vint4 a[2][TM], b[2][TN];
-        auto read = [&](int buf, unsigned half, int kk) {
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-                b[buf][j] = fragment<T, BN, B_KC>(lds + half + BM * kStepBytes, (wn * TN + j) * 32, kk, lane);
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-                a[buf][i] = fragment<T, BM, A_KC>(lds + half, (wm * TM + i) * 32, kk, lane);
+        constexpr int RING = 4, AHEAD = 3, GROUPS = 2 * TM, LAST = GROUPS - AHEAD;
+        static_assert(GROUPS % RING == 0, "the ring closes with the step");
+        vint4 a[RING], b[2][TN];
+        using FragmentA = Fragment<T, BM, A_KC>;
+        using FragmentB = Fragment<T, BN, B_KC>;
+        const unsigned lane_a = FragmentA::base(wm * TM * 16, lane);
+        const unsigned lane_b = FragmentB::base(wn * TN * 16, lane) + BM * kStepBytes;
+        unsigned at_a = lane_a, at_b = lane_b;
+        // the half that is read from now on; the addresses of single fragments are made where they are used (kept in
+        // registers they would not fit)
+        auto read_from = [&](unsigned half) {
+            at_a = lane_a + half;
+            at_b = lane_b + half;
+            asm("" : "+v"(at_a), "+v"(at_b));
         };
-        auto quarter = [&](int buf) {
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = multiply<T>(a[buf][i], b[buf][j], acc[i][j]);
-            interleave<kReads, kMfma, (kReads < kMfma ? kReads : kMfma)>();
+        auto read_a = [&](int group) { a[group % RING] = FragmentA::read(lds, at_a, group % TM, group / TM); };
+        auto read_b = [&](int kk, int j) { b[kk][j] = FragmentB::read(lds, at_b, j, kk); };
+        vint4 ra, rb;
+        unsigned ka[2], kb[2], to = 0;
+        constexpr int kCalls = LoadA::kCalls + LoadB::kCalls;
+        auto aim = [&](int s, unsigned at) {
+            la.aim(s, ra, ka);
+            lb.aim(s, rb, kb);
+            to = lds0 + at;
         };
+        auto call = [&](int c) {
+            if (c < LoadA::kCalls) la.call(c, ra, ka, to, wave);
+            else lb.call(c - LoadA::kCalls, rb, kb, to + BM * kStepBytes, wave);
+        };
+        auto group = [&](int g) {
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[g % TM][j] = multiply<T>(a[g % RING], b[g / TM][j], acc[g % TM][j]);
+        };
+        aim(s0, 0);
+#pragma unroll
+        for (int c = 0; c < kCalls; ++c) call(c);
+        if constexpr (MODE == GW && sizeof(T) == 2)
+            add_label_remainders<T, BM, BN, WM, WN>(g, m0, n0, wm, wn, lane, acc);
         wait_and_meet();
-        unsigned now = 0;
         if (s0 + 1 < s1) {
-            la.fetch(s0 + 1, lds0 + kStage, wave);
-            lb.fetch(s0 + 1, lds0 + kStage + BM * kStepBytes, wave);
-        }
-        read(0, now, 0);
-        auto first_three = [&] {
+            aim(s0 + 1, kStage);
 #pragma unroll
-            for (int kk = 0; kk < 3; ++kk) {
-                read((kk + 1) & 1, now, kk + 1);
-                quarter(kk & 1);
+            for (int c = 0; c < kCalls; ++c) call(c);
+        }
+        unsigned now = 0;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) read_b(0, j);
+#pragma unroll
+        for (int g = 0; g < AHEAD; ++g) read_a(g);
+        auto most = [&] {
+#pragma unroll
+            for (int g = 0; g < LAST; ++g) {
+                read_a(g + AHEAD);
+                if (g < TM) {
+#pragma unroll
+                    for (int j = TN * g / TM; j < TN * (g + 1) / TM; ++j) read_b(1, j);
+                }
+                group(g);
+                __builtin_amdgcn_sched_barrier(0);
             }
         };
         for (int s = s0; s + 1 < s1; ++s) {
-            first_three();
+            most();
             wait_and_meet();
-            if (s + 2 < s1) {
-                la.fetch(s + 2, lds0 + now, wave);
-                lb.fetch(s + 2, lds0 + now + BM * kStepBytes, wave);
-            }
+            const bool more = s + 2 < s1;
+            if (more) aim(s + 2, now);
             now = kStage - now;
-            read(0, now, 0);
-            quarter(1);
+            read_from(now);
+#pragma unroll
+            for (int g = LAST; g < GROUPS; ++g) {
+                const int x = g - LAST;
+#pragma unroll
+                for (int j = TN * x / AHEAD; j < TN * (x + 1) / AHEAD; ++j) read_b(0, j);
+                read_a(x);
+                group(g);
+                if (more) {
+#pragma unroll
+                    for (int c = kCalls * x / AHEAD; c < kCalls * (x + 1) / AHEAD; ++c) call(c);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
-        first_three();
-        quarter(1);
+        most();
+#pragma unroll
+        for (int g = LAST; g < GROUPS; ++g) group(g);
     }
 
-    const int mw = m0 + wm * TM * 32 + (lane >> 5) * 4, nw = n0 + wn * TN * 32 + (lane & 31);
+    const int mw = m0 + wm * TM * 16 + (lane >> 4) * 4, nw = n0 + wn * TN * 16 + (lane & 15);
+    const int m_wave = m0 + wm * TM * 16;
     if constexpr (MODE == STATS) {
         wait_and_meet();
         float2 *red = reinterpret_cast<float2 *>(lds_raw);      // [wm][column]
+        const float scale = scale_of<T>(g.alpha);
+        const bool tail = m0 + BM > g.M;
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-            const int n = nw + j * 32;
+            const int n = nw + j * 16;
             const int want = n < boundN ? g.label[n] - g.first : -1;
-            float top = -INFINITY, hit = 0.0f;
-            bool has = false;
+            // the label's logit: few tiles hold one
+            if (__builtin_amdgcn_ballot_w64(want >= m_wave && want < m_wave + TM * 16 && want < g.M)) {
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
+                for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int m = mw + i * 32 + (r >> 2) * 8 + (r & 3);
-                    const float z = m < g.M ? g.alpha * acc[i][j][r] : -INFINITY;
-                    acc[i][j][r] = z;
-                    top = fmaxf(top, z);
-                    if (m == want && m < g.M) {
-                        hit = z;
-                        has = true;
-                    }
-                }
-            if (has) g.target[n] = hit;
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float from = top == -INFINITY ? 0.0f : top;
-            float sum = 0.0f;
+                    for (int r = 0; r < 4; ++r)
+                        if (mw + i * 16 + r == want && want < g.M) g.target[n] = g.alpha * acc[i][j][r];
+            }
+            float top = -INFINITY, sum = 0.0f;
+            if (!tail && g.alpha > 0.0f) {
+                // the maximum of the products is that of the logits
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
+                for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sum += exponential<T>(acc[i][j][r] - from);
+                    for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[i][j][r]);
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float from = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sum += exponential<T>((acc[i][j][r] - from) * scale);
+                top *= g.alpha;
+            } else {
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (mw + i * 16 + r < g.M) top = fmaxf(top, g.alpha * acc[i][j][r]);
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float from = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (mw + i * 16 + r < g.M)
+                            sum += exponential<T>((g.alpha * acc[i][j][r] - from) * scale_of<T>(1.0f));
+            }
+            sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
-            if (lane < 32) red[wm * BN + (wn * TN + j) * 32 + lane] = make_float2(top, sum);
+            if (lane < 16) red[wm * BN + (wn * TN + j) * 16 + lane] = make_float2(top, sum);
         }
         __syncthreads();
         for (int c = threadIdx.x; c < BN; c += kThreads) {
@@ -457,101 +626,116 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
             for (int w = 0; w < WM; ++w) top = fmaxf(top, red[w * BN + c].x);
             const float from = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-            for (int w = 0; w < WM; ++w) {
-                const float t = red[w * BN + c].x;
-                sum += red[w * BN + c].y * exponential<T>((t == -INFINITY ? 0.0f : t) - from);
-            }
+            for (int w = 0; w < WM; ++w) sum += red[w * BN + c].y * expf(red[w * BN + c].x - from);
             if (n0 + c < boundN) g.stats[(int64_t)tm * g.ldStats + n0 + c] = make_float2(top, sum);
         }
     } else if constexpr (MODE == PROB) {
-        // Rounded to the operands' type, since the two products that follow run on it: each element is off by
-        // at most half a step (bf16: 2^-9 of itself), and the sums over tokens or vocabulary average that out.
-        T *P = static_cast<T *>(g.P);
+        // P is rounded to the operands' type, since the two products that follow run on it: each element is off
+        // by at most half a step of that type, and the sums over tokens or vocabulary average that out - except
+        // at the label, whose element outweighs the others: what its rounding took is kept (bf16) and goes into
+        // both products in fp32.  Past the last token and the last vocabulary row the tile is zeros, which the
+        // products may run into.
+        unsigned char *P = static_cast<unsigned char *>(g.P);
+        const float scale = scale_of<T>(g.alpha);
+        const bool tail = m0 + BM > g.M;
         if constexpr (sizeof(T) == 2) wait_and_meet();
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-            const int n = nw + j * 32;
-            if (n >= boundN) continue;
-            const float lse = g.lse[n], both = g.both[n], gloss = g.gloss[n];
-            const int want = g.label[n] - g.first;
+            const int n = nw + j * 16;
+            const bool live_n = n < boundN;
+            const float lse = live_n ? g.lse[n] * scale_of<T>(1.0f) : 0.0f, both = live_n ? g.both[n] : 0.0f;
+            const int want = live_n ? g.label[n] - g.first : -1;
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int m = mw + i * 32 + q * 8;
-                    T v[4];
+                for (int r = 0; r < 4; ++r) acc[i][j][r] = exponential<T>(fmaf(acc[i][j][r], scale, -lse)) * both;
+            if (__builtin_amdgcn_ballot_w64(want >= m_wave && want < m_wave + TM * 16)) {
+                const float gloss = live_n ? g.gloss[n] : 0.0f;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float p = exponential<T>(g.alpha * acc[i][j][4 * q + r] - lse) * both;
-                        if (m + r == want) p -= gloss;
-                        v[r] = from_float<T>(m + r < g.M ? p : 0.0f);
-                    }
-                    if constexpr (sizeof(T) == 2) {
-                        *reinterpret_cast<vint2 *>(lds_raw + staged_at<BM>(n - n0, m - m0)) =
-                            *reinterpret_cast<vint2 *>(v);
-                    } else {
-                        *reinterpret_cast<vint4 *>(P + (int64_t)n * g.ldP + m) = *reinterpret_cast<vint4 *>(v);
-                    }
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (mw + i * 16 + r == want) {
+                            const float p = acc[i][j][r] - gloss;
+                            acc[i][j][r] = p;
+                            if constexpr (sizeof(T) == 2) g.delta[g.rank[n]] = p - to_float(from_float<T>(p));
+                        }
+            }
+            if (tail || n0 + BN > boundN) {
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (!live_n || mw + i * 16 + r >= g.M) acc[i][j][r] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const int m = mw + i * 16;
+                T v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = from_float<T>(acc[i][j][r]);
+                if constexpr (sizeof(T) == 2) {
+                    *reinterpret_cast<vint2 *>(lds_raw + staged_at<BM>(n - n0, m - m0)) = *reinterpret_cast<vint2 *>(v);
+                } else {
+                    *reinterpret_cast<vint4 *>(P + p_byte<T>(n, m, g.ldP)) = *reinterpret_cast<vint4 *>(v);
                 }
+            }
         }
         if constexpr (sizeof(T) == 2) {
             __syncthreads();
-            write_staged<BM, kThreads>(lds_raw, P + (int64_t)n0 * g.ldP + m0, g.ldP,
-                                       boundN - n0 < BN ? boundN - n0 : BN, BM, true);
+            for (int i = threadIdx.x; i < BN * (BM / 8); i += kThreads) {       // along the rows of a block, block by block
+                const int row = i / 8 % BN, col = i / 8 / BN * kStep<T> + i % 8 * 8;
+                *reinterpret_cast<vint4 *>(P + p_byte<T>(n0 + row, m0 + col, g.ldP)) =
+                    *reinterpret_cast<const vint4 *>(lds_raw + staged_at<BM>(row, col));
+            }
         }
     } else if constexpr (MODE == GX) {
         float *part = g.part + (int64_t)blockIdx.y * g.splitStride;
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-            const int n = nw + j * 32;
+            const int n = nw + j * 16;
             if (n >= boundN) continue;
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int m = mw + i * 32 + q * 8;
-                    if (m >= g.M) continue;         // ldD is a multiple of 4: four fit where one does
-                    vfloat4 *to = reinterpret_cast<vfloat4 *>(part + (int64_t)n * g.ldD + m);
-                    vfloat4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                    if (g.add) {
-                        const vfloat4 old = *to;
-                        v += old;
-                    }
-                    *to = v;
+            for (int i = 0; i < TM; ++i) {
+                const int m = mw + i * 16;
+                if (m >= g.M) continue;         // ldD is a multiple of 4: four fit where one does
+                vfloat4 *to = reinterpret_cast<vfloat4 *>(part + (int64_t)n * g.ldD + m);
+                vfloat4 v = acc[i][j];
+                if (g.add) {
+                    const vfloat4 old = *to;
+                    v += old;
                 }
+                *to = v;
+            }
         }
     } else {
         T *out = static_cast<T *>(g.out);
         if constexpr (sizeof(T) == 2) wait_and_meet();
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-            const int n = nw + j * 32;
+            const int n = nw + j * 16;
             if (n >= boundN) continue;
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
+            for (int i = 0; i < TM; ++i) {
+                const int m = mw + i * 16;
+                T *to = out + (int64_t)n * g.ldD + m;
+                T v[4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int m = mw + i * 32 + q * 8;
-                    T *to = out + (int64_t)n * g.ldD + m;
-                    float x[4];
-                    T v[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        x[r] = acc[i][j][4 * q + r];
-                        if (g.beta != 0.0f && m + r < g.M) x[r] += g.beta * to_float(to[r]);
-                        v[r] = from_float<T>(x[r]);
-                    }
-                    if constexpr (sizeof(T) == 2) {
-                        *reinterpret_cast<vint2 *>(lds_raw + staged_at<BM>(n - n0, m - m0)) =
-                            *reinterpret_cast<vint2 *>(v);
-                    } else if (g.wide_out && m + 4 <= g.M) {
-                        *reinterpret_cast<vint4 *>(to) = *reinterpret_cast<vint4 *>(v);
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (m + r < g.M) to[r] = v[r];
-                    }
+                for (int r = 0; r < 4; ++r) {
+                    float x = acc[i][j][r];
+                    if (g.beta != 0.0f && m + r < g.M) x += g.beta * to_float(to[r]);
+                    v[r] = from_float<T>(x);
                 }
+                if constexpr (sizeof(T) == 2) {
+                    *reinterpret_cast<vint2 *>(lds_raw + staged_at<BM>(n - n0, m - m0)) = *reinterpret_cast<vint2 *>(v);
+                } else if (g.wide_out && m + 4 <= g.M) {
+                    *reinterpret_cast<vint4 *>(to) = *reinterpret_cast<vint4 *>(v);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (m + r < g.M) to[r] = v[r];
+                }
+            }
         }
         if constexpr (sizeof(T) == 2) {
             __syncthreads();
