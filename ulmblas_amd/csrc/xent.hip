@@ -151,36 +151,42 @@ gather_kernel(const T *__restrict__ src, int64_t ld, int cols, const int *rows, 
     }
 }
 
-// lse and loss of every compact token from the statistics of the tiles: 64
-// tokens a workgroup, four threads each.
+// lse and loss of every compact token from the statistics of the tiles: 16
+// tokens a workgroup, 16 threads each.
 template <typename T>
 __global__ void __launch_bounds__(256)
 loss_kernel(int tiles, const float2 *__restrict__ stats, int64_t ld, const float *__restrict__ target,
             const int *__restrict__ rows, const int *__restrict__ count, float *loss, float *lse)
 {
-    __shared__ float2 part[4][64];
+    __shared__ float2 part[16][16];
     const int live = *count;
-    if ((int)blockIdx.x * 64 >= live) return;
-    const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
-    const int c = blockIdx.x * 64 + lane;
+    if ((int)blockIdx.x * 16 >= live) return;
+    const int token = threadIdx.x & 15, slice = threadIdx.x >> 4;
+    const int c = blockIdx.x * 16 + token;
     float top = -INFINITY, sum = 0.0f;
     if (c < live) {
-        for (int i = slice; i < tiles; i += 4) {
-            const float2 s = stats[i * ld + c];
-            const float t = fmaxf(top, s.x);
-            const float from = t == -INFINITY ? 0.0f : t;
-            // an empty side has sum 0 and maximum -inf: exp(-inf) times 0
-            sum = sum * expf(top - from) + s.y * expf(s.x - from);
-            top = t;
+        for (int i0 = slice; i0 < tiles; i0 += 64) {
+            float2 s[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                s[u] = i0 + 16 * u < tiles ? stats[(i0 + 16 * u) * ld + c] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float t = fmaxf(top, s[u].x);
+                const float from = t == -INFINITY ? 0.0f : t;
+                // an empty side has sum 0 and maximum -inf: exp(-inf) times 0
+                sum = sum * expf(top - from) + s[u].y * expf(s[u].x - from);
+                top = t;
+            }
         }
     }
-    part[slice][lane] = make_float2(top, sum);
+    part[slice][token] = make_float2(top, sum);
     __syncthreads();
     if (slice == 0 && c < live) {
-        for (int k = 1; k < 4; ++k) top = fmaxf(top, part[k][lane].x);
+        for (int k = 1; k < 16; ++k) top = fmaxf(top, part[k][token].x);
         const float from = top == -INFINITY ? 0.0f : top;
         sum = 0.0f;
-        for (int k = 0; k < 4; ++k) sum += part[k][lane].y * expf(part[k][lane].x - from);
+        for (int k = 0; k < 16; ++k) sum += part[k][token].y * expf(part[k][token].x - from);
         const float l = from + logf(sum);
         const int t = rows[c];
         lse[t] = l;
@@ -189,23 +195,39 @@ loss_kernel(int tiles, const float2 *__restrict__ stats, int64_t ld, const float
 }
 
 // gX of every row: the sum over the splits in order (bf16: and what rounding
-// took from P at the label), or zeros.
+// took from P at the label), or zeros.  Four elements a thread.
 template <typename T>
 __global__ void __launch_bounds__(256)
 gx_kernel(int hidden, const int *__restrict__ place, const float *__restrict__ part, int64_t ld, int64_t stride,
-          int splits, const float *__restrict__ delta, const int *__restrict__ rank, const int *__restrict__ label, const T *__restrict__ W, int64_t ldw,
-          T *gx, int64_t ldgx)
+          int splits, const float *__restrict__ delta, const int *__restrict__ rank, const int *__restrict__ label,
+          const T *__restrict__ W, int64_t ldw, T *gx, int64_t ldgx)
 {
-    const int t = blockIdx.x, c = place[t];
-    T *to = gx + t * ldgx;
-    const float d = sizeof(T) == 2 && c >= 0 ? delta[rank[c]] : 0.0f;
-    const T *w = c >= 0 ? W + label[c] * ldw : W;
-    for (int h = threadIdx.x; h < hidden; h += 256) {
-        float v = sizeof(T) == 2 && c >= 0 ? d * to_float(w[h]) : 0.0f;
-        if (c >= 0)
-            for (int s = 0; s < splits; ++s) v += part[s * stride + c * ld + h];
-        to[h] = from_float<T>(v);
+    const int t = blockIdx.x, c = place[t], h = (int)(blockIdx.y * 256 + threadIdx.x) * 4;
+    if (h >= hidden) return;
+    const int n = hidden - h < 4 ? hidden - h : 4;
+    vfloat4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (c >= 0) {
+        if (sizeof(T) == 2) {
+            const float d = delta[rank[c]];
+            const T *w = W + label[c] * ldw + h;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = e < n ? d * to_float(w[e]) : 0.0f;
+        }
+        const float *p = part + c * ld + h;
+        int s = 0;
+        for (; s + 4 <= splits; s += 4) {
+            vfloat4 x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] = *reinterpret_cast<const vfloat4 *>(p + (s + u) * stride);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v += x[u];
+        }
+        for (; s < splits; ++s) v += *reinterpret_cast<const vfloat4 *>(p + s * stride);
     }
+    T *to = gx + t * ldgx + h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (e < n) to[e] = from_float<T>(v[e]);
 }
 
 // ---------------------------------------------------------------------------
@@ -218,64 +240,6 @@ constexpr int kMaxHidden = 1 << 20, kMaxRows = 1 << 28;
 std::atomic<int> g_piece_rows{0};
 
 inline int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
-
-// What the workspace holds and where; every part starts on 256 bytes.
-struct Layout {
-    int64_t tokens_p, hidden_p;         // rounded up: rows of compact copies, elements of their rows
-    int piece;                          // vocabulary rows at a time (gradient: of P; packing: of W)
-    int splits;                         // partial sums of gX
-    int64_t rows, label, place, lse, both, gloss, delta, target, bucket, member, rank, count, x, w, stats, p, part, bytes;
-};
-
-constexpr int64_t kPieceBytes = (int64_t)1 << 30;       // of P or of a packed copy of W, at the most
-
-template <typename T> Layout layout(int hidden, int tokens, int vocab, bool grad)
-{
-    Layout l{};
-    l.tokens_p = round_up(std::max(tokens, 1), 256);
-    l.hidden_p = round_up(hidden, kStep<T>);
-    const int64_t row = std::max(grad ? l.tokens_p : 0, l.hidden_p) * (int64_t)sizeof(T);
-    int64_t piece = std::max<int64_t>(kPieceBytes / row / 256 * 256, 256);
-    piece = std::min<int64_t>(piece, 1 << 19);
-    if (g_piece_rows.load() > 0) piece = std::min<int64_t>(piece, round_up(g_piece_rows.load(), 256));
-    l.piece = (int)std::min<int64_t>(piece, round_up(vocab, 256));
-    l.splits = 1;
-    if (grad) {
-        const int64_t tiles = (round_up(hidden, 128) / 128) * (l.tokens_p / 128);
-        l.splits = (int)std::min<int64_t>(8, std::max<int64_t>(1, 256 / tiles));
-        l.splits = (int)std::min<int64_t>(l.splits, std::max<int64_t>(1, l.piece / 1024));
-    }
-    int64_t at = 0;
-    auto take = [&](int64_t bytes) {
-        const int64_t here = at;
-        at += round_up(bytes, 256);
-        return here;
-    };
-    l.count = take(4);
-    l.rows = take(4 * l.tokens_p);
-    l.label = take(4 * l.tokens_p);
-    l.target = take(4 * l.tokens_p);
-    if (grad) {
-        l.place = take(4 * l.tokens_p);
-        l.lse = take(4 * l.tokens_p);
-        l.both = take(4 * l.tokens_p);
-        l.gloss = take(4 * l.tokens_p);
-        l.delta = take(4 * l.tokens_p);
-        l.member = take(8 * l.tokens_p);
-        l.rank = take(4 * l.tokens_p);
-        l.bucket = take(4 * (round_up(vocab, 128) / 128 + 1));
-    }
-    l.x = take(l.tokens_p * l.hidden_p * (int64_t)sizeof(T));
-    l.w = take((int64_t)l.piece * l.hidden_p * (int64_t)sizeof(T));
-    if (!grad) {
-        l.stats = take((round_up(vocab, 256) / 128) * l.tokens_p * 8);
-    } else {
-        l.p = take(l.tokens_p * l.piece * (int64_t)sizeof(T));
-        l.part = take((int64_t)l.splits * l.tokens_p * l.hidden_p * 4);
-    }
-    l.bytes = at;
-    return l;
-}
 
 bool sizes_ok(int hidden, int tokens, int vocab)
 {
@@ -311,21 +275,100 @@ int launch_tile(const ProductArgs &g, hipStream_t stream)
     return ULMBLAS_GPU_OK;
 }
 
-// The 256 x 256 tile where it fills most of the GPU's 256 CUs, else 128 x 128.
-bool large_tile(int M, int N) { return (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 200; }
+// The tile a product of M x N runs on.  N counts tokens in all products but GW.
+//  - up to 32 tokens: 128 x 32, of which four workgroups share a CU: the product is bound by the bytes of W then;
+//  - 256 x 256 where that fills most of the GPU's 256 CUs, with `splits` of k in GX;
+//  - else 128 x 128.
+enum Tile { NARROW, SMALL, LARGE };
+template <Mode MODE> Tile tile_for(int M, int N, int splits)
+{
+    if (MODE != GW && N <= 32) return NARROW;
+    return (int64_t)((M + 255) / 256) * ((N + 255) / 256) * splits >= 200 ? LARGE : SMALL;
+}
+int tile_rows(Tile t) { return t == LARGE ? 256 : 128; }
+
+// Into how many parts k of GX is cut: two rounds of workgroups if every token
+// has a target, as much as it takes with the small tile if there are few tiles.
+int splits_of_gx(int hidden, int tokens, int piece)
+{
+    const int64_t large = ((hidden + 255) / 256) * (int64_t)((tokens + 255) / 256);
+    const int64_t small = ((hidden + 127) / 128) * (int64_t)((tokens + 127) / 128);
+    const int64_t want = large >= 16 ? 512 / large : 512 / small;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 64), piece / 512));
+}
+
+// What the workspace holds and where; every part starts on 256 bytes.
+struct Layout {
+    int64_t tokens_p, hidden_p;         // rounded up: rows of compact copies, elements of their rows
+    int piece;                          // vocabulary rows at a time (gradient: of P; packing: of W)
+    int splits;                         // partial sums of gX
+    int64_t rows, label, place, lse, both, gloss, delta, target, bucket, member, rank, count, x, w, stats, p, part, bytes;
+};
+
+constexpr int64_t kPieceBytes = (int64_t)1 << 30;       // of P or of a packed copy of W, at the most
+
+template <typename T> Layout layout(int hidden, int tokens, int vocab, bool grad)
+{
+    Layout l{};
+    l.tokens_p = round_up(std::max(tokens, 1), 256);
+    l.hidden_p = round_up(hidden, kStep<T>);
+    const int64_t row = std::max(grad ? l.tokens_p : 0, l.hidden_p) * (int64_t)sizeof(T);
+    int64_t piece = std::max<int64_t>(kPieceBytes / row / 256 * 256, 256);
+    piece = std::min<int64_t>(piece, 1 << 19);
+    if (g_piece_rows.load() > 0) piece = std::min<int64_t>(piece, round_up(g_piece_rows.load(), 256));
+    l.piece = (int)std::min<int64_t>(piece, round_up(vocab, 256));
+    l.splits = 1;
+    if (grad) {
+        l.splits = splits_of_gx(hidden, std::max(tokens, 1), l.piece);
+    }
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += round_up(bytes, 256);
+        return here;
+    };
+    l.count = take(4);
+    l.rows = take(4 * l.tokens_p);
+    l.label = take(4 * l.tokens_p);
+    l.target = take(4 * l.tokens_p);
+    if (grad) {
+        l.place = take(4 * l.tokens_p);
+        l.lse = take(4 * l.tokens_p);
+        l.both = take(4 * l.tokens_p);
+        l.gloss = take(4 * l.tokens_p);
+        l.delta = take(4 * l.tokens_p);
+        l.member = take(8 * l.tokens_p);
+        l.rank = take(4 * l.tokens_p);
+        l.bucket = take(4 * (round_up(vocab, 128) / 128 + 1));
+    }
+    l.x = take(l.tokens_p * l.hidden_p * (int64_t)sizeof(T));
+    l.w = take((int64_t)l.piece * l.hidden_p * (int64_t)sizeof(T));
+    if (!grad) {
+        l.stats = take((round_up(vocab, 256) / 128) * l.tokens_p * 8);
+    } else {
+        l.p = take(l.tokens_p * l.piece * (int64_t)sizeof(T));
+        l.part = take((int64_t)l.splits * l.tokens_p * l.hidden_p * 4);
+    }
+    l.bytes = at;
+    return l;
+}
 
 template <typename T, Mode MODE> int launch_product(const ProductArgs &g, hipStream_t stream)
 {
-    if (large_tile(g.M, g.N)) return launch_tile<T, MODE, 256, 256, 2, 4>(g, stream);
-    return launch_tile<T, MODE, 128, 128, 2, 2>(g, stream);
+    switch (tile_for<MODE>(g.M, g.N, MODE == GX ? g.splits : 1)) {
+    case LARGE: return launch_tile<T, MODE, 256, 256, 2, 4>(g, stream);
+    case SMALL: return launch_tile<T, MODE, 128, 128, 2, 2>(g, stream);
+    default:
+        if constexpr (MODE != GW) return launch_tile<T, MODE, 128, 32, 4, 1>(g, stream);
+        return ULMBLAS_GPU_BAD_ARGUMENT;        // GW has no narrow tile
+    }
 }
 
-// Whether the product kernel can read W where it lies: rows on 16 bytes, no
-// row ending inside 16 bytes, and a tile's rows within 31 bits of each other.
-template <typename T> bool in_place(const T *W, int ldW, int hidden)
+// Whether the product kernel can read W where it lies: rows that start on 4
+// bytes, and a tile's rows within 31 bits of each other.
+template <typename T> bool in_place(const T *W, int ldW)
 {
-    return ((uintptr_t)W & 15) == 0 && ldW * sizeof(T) % 16 == 0 && hidden * sizeof(T) % 16 == 0 &&
-           (int64_t)ldW * (int64_t)sizeof(T) < (1 << 23);
+    return ((uintptr_t)W & 3) == 0 && ldW * sizeof(T) % 4 == 0 && (int64_t)ldW * (int64_t)sizeof(T) < (1 << 23);
 }
 
 template <typename T>
@@ -383,7 +426,7 @@ int xent_device(int hidden, int tokens, int vocab, float alpha, const T *W, int 
     g.label = t.label_c;
     g.ldStats = l.tokens_p;
     g.target = part_of<float>(work, l.target);
-    const bool direct = in_place(W, ldW, hidden);
+    const bool direct = in_place(W, ldW);
     const int piece = direct ? vocab : l.piece;
     int tiles = 0;
     for (int v0 = 0; v0 < vocab; v0 += piece) {
@@ -403,10 +446,10 @@ int xent_device(int hidden, int tokens, int vocab, float alpha, const T *W, int 
         }
         g.stats = part_of<float2>(work, l.stats) + (int64_t)tiles * l.tokens_p;
         if ((rc = launch_product<T, STATS>(g, stream))) return rc;
-        const int bm = large_tile(g.M, g.N) ? 256 : 128;
+        const int bm = tile_rows(tile_for<STATS>(g.M, g.N, 1));
         tiles += (g.M + bm - 1) / bm;
     }
-    hipLaunchKernelGGL(loss_kernel<T>, dim3((unsigned)((tokens + 63) / 64)), dim3(256), 0, stream, tiles,
+    hipLaunchKernelGGL(loss_kernel<T>, dim3((unsigned)((tokens + 15) / 16)), dim3(256), 0, stream, tiles,
                        part_of<float2>(work, l.stats), l.tokens_p, g.target, t.rows, t.count, loss, lse);
     HIP_TRY(hipGetLastError());
     return ULMBLAS_GPU_OK;
@@ -457,7 +500,7 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
     // P: rows of blocks; all of them
     const int64_t row_x = l.hidden_p * (int64_t)sizeof(T), row_p = (int64_t)l.piece / kStep<T> * kBlockBytes;
     const int blocks_p = (int)(l.tokens_p / kBlockTokens * (l.piece / kStep<T>));
-    const bool direct = in_place(W, ldW, hidden);
+    const bool direct = in_place(W, ldW);
     for (int v0 = 0; v0 < vocab; v0 += l.piece) {
         const int vn = std::min(l.piece, vocab - v0);
         const T *Wv = W ? W + (int64_t)v0 * ldW : nullptr;
@@ -528,12 +571,11 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
             g.out = gW + (int64_t)v0 * ldGW;
             g.ldD = ldGW;
             g.beta = beta;
-            g.wide_out = (uintptr_t)g.out % 16 == 0 && ldGW * sizeof(T) % 16 == 0;
             if ((rc = launch_product<T, GW>(g, stream))) return rc;
         }
     }
     if (gX && tokens > 0) {
-        hipLaunchKernelGGL(gx_kernel<T>, dim3((unsigned)tokens), dim3(256), 0, stream, hidden, t.place,
+        hipLaunchKernelGGL(gx_kernel<T>, dim3((unsigned)tokens, (unsigned)((hidden + 1023) / 1024)), dim3(256), 0, stream, hidden, t.place,
                            part_of<float>(work, l.part), l.hidden_p, l.tokens_p * l.hidden_p, l.splits, delta, rank,
                            t.label_c, W, (int64_t)ldW, gX,
                            (int64_t)ldGX);

@@ -110,7 +110,6 @@ struct ProductArgs {
     // GW
     void *out;
     float beta;
-    int wide_out;               // rows of out lie on 16 bytes
     const int *bucket;          // first place of each group of 128 vocabulary rows
     const int2 *member;         // tokens (compact) in the order of their label's group, and their labels
 };
@@ -152,7 +151,8 @@ struct Loader {
         ld = ld_;
         int64_t total, skip;
         if constexpr (LIE == ALONG || LIE == ACROSS) {
-            total = rows > 0 ? (int64_t)(rows - 1) * ld + (int64_t)width * (int64_t)sizeof(T) : 0;
+            // whole words: the buffer's range would cut off half of an odd row's last one
+            total = rows > 0 ? ((int64_t)(rows - 1) * ld + (int64_t)width * (int64_t)sizeof(T) + 3) & ~(int64_t)3 : 0;
             skip = LIE == ALONG ? (int64_t)row0 * ld : (int64_t)row0 * (int64_t)sizeof(T);
         } else {
             total = (int64_t)width * kBlockBytes;
@@ -341,29 +341,25 @@ template <int BM> __device__ __forceinline__ int staged_at(int row, int col)
     return row * (BM * 2) + (((col >> 3) ^ (row & (kChunks - 1))) << 4) + (col & 7) * 2;
 }
 
-// Writes the staged tile out, whole rows at a time: rows x cols of it, 16 bytes
-// a lane where the rows lie on 16 bytes, else element by element.
+// 16 bytes at whatever address its elements have.
+template <typename T> struct AnyVector;
+template <> struct AnyVector<bf16_t> { typedef vint4 V __attribute__((aligned(2))); };
+template <> struct AnyVector<float> { typedef vint4 V __attribute__((aligned(4))); };
+
+// Writes the staged tile out, whole rows at a time: rows x cols of it.
 template <int BM, int THREADS>
-__device__ __forceinline__ void write_staged(const unsigned char *lds, bf16_t *to, int64_t ld, int rows, int cols,
-                                             bool wide)
+__device__ __forceinline__ void write_staged(const unsigned char *lds, bf16_t *to, int64_t ld, int rows, int cols)
 {
     constexpr int kChunks = BM / 8;
-    if (wide) {
-        for (int i = threadIdx.x; i < rows * kChunks; i += THREADS) {
-            const int row = i / kChunks, col = i % kChunks * 8;
-            if (col >= cols) continue;
-            const unsigned char *v = lds + staged_at<BM>(row, col);
-            bf16_t *p = to + row * ld + col;
-            if (col + 8 <= cols) {
-                *reinterpret_cast<vint4 *>(p) = *reinterpret_cast<const vint4 *>(v);
-            } else {
-                for (int e = 0; e < cols - col; ++e) p[e] = reinterpret_cast<const bf16_t *>(v)[e];
-            }
-        }
-    } else {
-        for (int i = threadIdx.x; i < rows * BM; i += THREADS) {
-            const int row = i / BM, col = i % BM;
-            if (col < cols) to[row * ld + col] = *reinterpret_cast<const bf16_t *>(lds + staged_at<BM>(row, col));
+    for (int i = threadIdx.x; i < rows * kChunks; i += THREADS) {
+        const int row = i / kChunks, col = i % kChunks * 8;
+        if (col >= cols) continue;
+        const unsigned char *v = lds + staged_at<BM>(row, col);
+        bf16_t *p = to + row * ld + col;
+        if (col + 8 <= cols) {
+            *reinterpret_cast<AnyVector<bf16_t>::V *>(p) = *reinterpret_cast<const vint4 *>(v);
+        } else {
+            for (int e = 0; e < cols - col; ++e) p[e] = reinterpret_cast<const bf16_t *>(v)[e];
         }
     }
 }
@@ -478,7 +474,7 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
     // be refilled for the step after next, and the matrix cores have work while
     // the waves meet and the next step's first fragments come out of LDS.
     if (s0 < s1) {
-        constexpr int RING = 4, AHEAD = 3, GROUPS = 2 * TM, LAST = GROUPS - AHEAD;
+        constexpr int RING = 4, AHEAD = 3, GROUPS = 2 * TM, LAST = GROUPS - AHEAD, SPREAD = TM < LAST ? TM : LAST;
         static_assert(GROUPS % RING == 0, "the ring closes with the step");
         vint4 a[RING], b[2][TN];
         using FragmentA = Fragment<T, BM, A_KC>;
@@ -507,9 +503,13 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
             if (c < LoadA::kCalls) la.call(c, ra, ka, to, wave);
             else lb.call(c - LoadA::kCalls, rb, kb, to + BM * kStepBytes, wave);
         };
-        auto group = [&](int g) {
+        // In the last step a chunk of a row of A may run past the row's end, into whatever follows it.
+        vint4 valid[2];
+        auto group = [&](int g, bool last) {
+            vint4 x = a[g % RING];
+            if (LIE_A == ALONG && last) x &= valid[g / TM];
 #pragma unroll
-            for (int j = 0; j < TN; ++j) acc[g % TM][j] = multiply<T>(a[g % RING], b[g / TM][j], acc[g % TM][j]);
+            for (int j = 0; j < TN; ++j) acc[g % TM][j] = multiply<T>(x, b[g / TM][j], acc[g % TM][j]);
         };
         aim(s0, 0);
 #pragma unroll
@@ -527,20 +527,20 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
         for (int j = 0; j < TN; ++j) read_b(0, j);
 #pragma unroll
         for (int g = 0; g < AHEAD; ++g) read_a(g);
-        auto most = [&] {
+        auto most = [&](bool last) {
 #pragma unroll
             for (int g = 0; g < LAST; ++g) {
                 read_a(g + AHEAD);
-                if (g < TM) {
+                if (g < SPREAD) {
 #pragma unroll
-                    for (int j = TN * g / TM; j < TN * (g + 1) / TM; ++j) read_b(1, j);
+                    for (int j = TN * g / SPREAD; j < TN * (g + 1) / SPREAD; ++j) read_b(1, j);
                 }
-                group(g);
+                group(g, last);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
         for (int s = s0; s + 1 < s1; ++s) {
-            most();
+            most(false);
             wait_and_meet();
             const bool more = s + 2 < s1;
             if (more) aim(s + 2, now);
@@ -552,7 +552,7 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
 #pragma unroll
                 for (int j = TN * x / AHEAD; j < TN * (x + 1) / AHEAD; ++j) read_b(0, j);
                 read_a(x);
-                group(g);
+                group(g, false);
                 if (more) {
 #pragma unroll
                     for (int c = kCalls * x / AHEAD; c < kCalls * (x + 1) / AHEAD; ++c) call(c);
@@ -560,9 +560,20 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        most();
+        if constexpr (LIE_A == ALONG) {
 #pragma unroll
-        for (int g = LAST; g < GROUPS; ++g) group(g);
+            for (int kk = 0; kk < 2; ++kk) {
+                const int have = K - (s1 - 1) * kStep<T> - (4 * kk + (lane >> 4)) * (16 / (int)sizeof(T));
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    if constexpr (sizeof(T) == 2) valid[kk][w] = have > 2 * w + 1 ? -1 : have > 2 * w ? 0xffff : 0;
+                    else valid[kk][w] = have > w ? -1 : 0;
+                }
+            }
+        }
+        most(true);
+#pragma unroll
+        for (int g = LAST; g < GROUPS; ++g) group(g, true);
     }
 
     const int mw = m0 + wm * TM * 16 + (lane >> 4) * 4, nw = n0 + wn * TN * 16 + (lane & 15);
@@ -683,10 +694,13 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
         }
         if constexpr (sizeof(T) == 2) {
             __syncthreads();
-            for (int i = threadIdx.x; i < BN * (BM / 8); i += kThreads) {       // along the rows of a block, block by block
-                const int row = i / 8 % BN, col = i / 8 / BN * kStep<T> + i % 8 * 8;
-                *reinterpret_cast<vint4 *>(P + p_byte<T>(n0 + row, m0 + col, g.ldP)) =
-                    *reinterpret_cast<const vint4 *>(lds_raw + staged_at<BM>(row, col));
+            // along the rows of a block, block by block; GW takes rows in steps, which a narrow tile does not fill
+            constexpr int kRows = BN < kStep<T> ? kStep<T> : BN;
+            for (int i = threadIdx.x; i < kRows * (BM / 8); i += kThreads) {
+                const int row = i / 8 % kRows, col = i / 8 / kRows * kStep<T> + i % 8 * 8;
+                vint4 v = {0, 0, 0, 0};
+                if (row < BN) v = *reinterpret_cast<const vint4 *>(lds_raw + staged_at<BM>(row, col));
+                *reinterpret_cast<vint4 *>(P + p_byte<T>(n0 + row, m0 + col, g.ldP)) = v;
             }
         }
     } else if constexpr (MODE == GX) {
@@ -728,8 +742,8 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
                 }
                 if constexpr (sizeof(T) == 2) {
                     *reinterpret_cast<vint2 *>(lds_raw + staged_at<BM>(n - n0, m - m0)) = *reinterpret_cast<vint2 *>(v);
-                } else if (g.wide_out && m + 4 <= g.M) {
-                    *reinterpret_cast<vint4 *>(to) = *reinterpret_cast<vint4 *>(v);
+                } else if (m + 4 <= g.M) {
+                    *reinterpret_cast<AnyVector<float>::V *>(to) = *reinterpret_cast<vint4 *>(v);
                 } else {
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
@@ -740,7 +754,7 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
         if constexpr (sizeof(T) == 2) {
             __syncthreads();
             write_staged<BM, kThreads>(lds_raw, out + (int64_t)n0 * g.ldD + m0, g.ldD, g.N - n0 < BN ? g.N - n0 : BN,
-                                       g.M - m0 < BM ? g.M - m0 : BM, g.wide_out);
+                                       g.M - m0 < BM ? g.M - m0 : BM);
         }
     }
 }
