@@ -43,6 +43,32 @@ struct TokenArgs {
     float *lse_c, *both_c, *gloss_c;
 };
 
+// The label of row t, or -1 if it is none.
+__device__ __forceinline__ int target_of(const TokenArgs &g, int t)
+{
+    const int y = g.label[t];
+    return y == g.ignore || y < 0 || y >= g.vocab ? -1 : y;
+}
+
+// Row t has label y and compact place c, or no target (y < 0).
+__device__ __forceinline__ void note_row(const TokenArgs &g, int t, int y, int c)
+{
+    if (y >= 0) {
+        g.rows[c] = t;
+        g.label_c[c] = y;
+        if (g.lse) {
+            const float gl = g.gloss[t];
+            g.lse_c[c] = g.lse[t];
+            g.gloss_c[c] = g.alpha * gl;
+            g.both_c[c] = g.alpha * (g.glse ? gl + g.glse[t] : gl);
+        }
+    } else if (g.loss) {
+        g.loss[t] = 0.0f;
+        g.lse_out[t] = 0.0f;
+    }
+    if (g.place) g.place[t] = y >= 0 ? c : -1;
+}
+
 // One workgroup: which rows have a target, in order.
 __global__ void __launch_bounds__(1024) token_kernel(TokenArgs g)
 {
@@ -51,11 +77,7 @@ __global__ void __launch_bounds__(1024) token_kernel(TokenArgs g)
     int done = 0;
     for (int t0 = 0; t0 < g.tokens; t0 += 1024) {
         const int t = t0 + (int)threadIdx.x;
-        int y = -1;
-        if (t < g.tokens) {
-            y = g.label[t];
-            if (y == g.ignore || y < 0 || y >= g.vocab) y = -1;
-        }
+        const int y = t < g.tokens ? target_of(g, t) : -1;
         const unsigned long long votes = __builtin_amdgcn_ballot_w64(y >= 0);
         if (lane == 0) wave_sum[wave] = __popcll(votes);
         __syncthreads();
@@ -65,20 +87,7 @@ __global__ void __launch_bounds__(1024) token_kernel(TokenArgs g)
             all += wave_sum[w];
         }
         const int c = before + __popcll(votes & ((1ull << lane) - 1));
-        if (y >= 0) {
-            g.rows[c] = t;
-            g.label_c[c] = y;
-            if (g.lse) {
-                const float gl = g.gloss[t];
-                g.lse_c[c] = g.lse[t];
-                g.gloss_c[c] = g.alpha * gl;
-                g.both_c[c] = g.alpha * (g.glse ? gl + g.glse[t] : gl);
-            }
-        } else if (t < g.tokens && g.loss) {
-            g.loss[t] = 0.0f;
-            g.lse_out[t] = 0.0f;
-        }
-        if (g.place && t < g.tokens) g.place[t] = y >= 0 ? c : -1;
+        if (t < g.tokens) note_row(g, t, y, c);
         done = all;
         __syncthreads();
     }
@@ -126,8 +135,22 @@ bucket_kernel(const int *__restrict__ count, const int *__restrict__ label, int2
     }
 }
 
-// dst[c] <- src[rows ? rows[c] : c], padded with zeros to `width` elements.
-// One workgroup a row.
+// One row into its place, padded with zeros to `width` elements, by a workgroup.
+template <typename T>
+__device__ __forceinline__ void copy_row(const T *__restrict__ from, int cols, T *__restrict__ to, int64_t width)
+{
+    using V = typename AnyVector<T>::V;
+    constexpr int N = 16 / sizeof(T);
+    for (int64_t i = threadIdx.x * N; i < width; i += 256 * N) {
+        if (i + N <= cols) {
+            *reinterpret_cast<vint4 *>(to + i) = *reinterpret_cast<const V *>(from + i);
+        } else {
+            for (int e = 0; e < N; ++e) to[i + e] = i + e < cols ? from[i + e] : T(0);
+        }
+    }
+}
+
+// dst[c] <- src[rows ? rows[c] : c].  One workgroup a row.
 template <typename T>
 __global__ void __launch_bounds__(256)
 gather_kernel(const T *__restrict__ src, int64_t ld, int cols, const int *rows, const int *count, T *__restrict__ dst,
@@ -135,59 +158,73 @@ gather_kernel(const T *__restrict__ src, int64_t ld, int cols, const int *rows, 
 {
     const int c = blockIdx.x;
     if (count && c >= *count) return;
-    const T *from = src + (rows ? rows[c] : c) * ld;
-    T *to = dst + c * width;
-    constexpr int V = 16 / sizeof(T);
-    if (((uintptr_t)from & 15) == 0) {
-        for (int64_t i = threadIdx.x * V; i < width; i += 256 * V) {
-            if (i + V <= cols) {
-                *reinterpret_cast<vint4 *>(to + i) = *reinterpret_cast<const vint4 *>(from + i);
-            } else {
-                for (int e = 0; e < V; ++e) to[i + e] = i + e < cols ? from[i + e] : T(0);
-            }
-        }
-    } else {
-        for (int64_t i = threadIdx.x; i < width; i += 256) to[i] = i < cols ? from[i] : T(0);
-    }
+    copy_row<T>(src + (rows ? rows[c] : c) * ld, cols, dst + c * width, width);
 }
 
-// lse and loss of every compact token from the statistics of the tiles: 16
-// tokens a workgroup, 16 threads each.
+// Both at once for few rows: a workgroup a row, which finds its place by
+// counting the targets before it.
 template <typename T>
+__global__ void __launch_bounds__(256)
+token_gather_kernel(TokenArgs g, const T *__restrict__ src, int64_t ld, int cols, T *__restrict__ dst, int64_t width)
+{
+    __shared__ int wave_sum[4];
+    const int t = blockIdx.x, y = target_of(g, t);
+    int before = 0;
+    for (int i = threadIdx.x; i < t; i += 256) before += target_of(g, i) >= 0;
+    for (int d = 32; d; d >>= 1) before += __shfl_xor(before, d);
+    if ((threadIdx.x & 63) == 0) wave_sum[threadIdx.x >> 6] = before;
+    __syncthreads();
+    const int c = wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
+    if (threadIdx.x == 0) {
+        note_row(g, t, y, c);
+        if (t == g.tokens - 1) *g.count = c + (y >= 0);
+    }
+    if (y >= 0) copy_row<T>(src + t * ld, cols, dst + c * width, width);
+}
+
+// lse and loss of every compact token from the statistics of the tiles:
+// 2^SHIFT tokens a workgroup, the other threads share the tiles.
+template <typename T, int SHIFT>
 __global__ void __launch_bounds__(256)
 loss_kernel(int tiles, const float2 *__restrict__ stats, int64_t ld, const float *__restrict__ target,
             const int *__restrict__ rows, const int *__restrict__ count, float *loss, float *lse)
 {
-    __shared__ float2 part[16][16];
+    constexpr int TOKENS = 1 << SHIFT, SLICES = 256 >> SHIFT;
+    __shared__ float2 part[SLICES][TOKENS];
     const int live = *count;
-    if ((int)blockIdx.x * 16 >= live) return;
-    const int token = threadIdx.x & 15, slice = threadIdx.x >> 4;
-    const int c = blockIdx.x * 16 + token;
+    if ((int)blockIdx.x * TOKENS >= live) return;
+    const int token = threadIdx.x & (TOKENS - 1), slice = threadIdx.x >> SHIFT;
+    const int c = blockIdx.x * TOKENS + token;
     float top = -INFINITY, sum = 0.0f;
     if (c < live) {
-        for (int i0 = slice; i0 < tiles; i0 += 64) {
+        for (int i0 = slice; i0 < tiles; i0 += 4 * SLICES) {
             float2 s[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                s[u] = i0 + 16 * u < tiles ? stats[(i0 + 16 * u) * ld + c] : make_float2(-INFINITY, 0.0f);
+            float t = top;
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const float t = fmaxf(top, s[u].x);
-                const float from = t == -INFINITY ? 0.0f : t;
-                // an empty side has sum 0 and maximum -inf: exp(-inf) times 0
-                sum = sum * expf(top - from) + s[u].y * expf(s[u].x - from);
-                top = t;
+                s[u] = i0 + SLICES * u < tiles ? stats[(i0 + SLICES * u) * ld + c] : make_float2(-INFINITY, 0.0f);
+                t = fmaxf(t, s[u].x);
             }
+            const float from = t == -INFINITY ? 0.0f : t;
+            // an empty side has sum 0 and maximum -inf: exp(-inf) times 0
+            sum *= expf(top - from);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) sum += s[u].y * expf(s[u].x - from);
+            top = t;
         }
     }
     part[slice][token] = make_float2(top, sum);
-    __syncthreads();
+    for (int half = SLICES / 2; half >= 1; half /= 2) {
+        __syncthreads();
+        if (slice < half) {
+            const float2 a = part[slice][token], b = part[slice + half][token];
+            const float t = fmaxf(a.x, b.x), from = t == -INFINITY ? 0.0f : t;
+            part[slice][token] = make_float2(t, a.y * expf(a.x - from) + b.y * expf(b.x - from));
+        }
+    }
     if (slice == 0 && c < live) {
-        for (int k = 1; k < 16; ++k) top = fmaxf(top, part[k][token].x);
-        const float from = top == -INFINITY ? 0.0f : top;
-        sum = 0.0f;
-        for (int k = 0; k < 16; ++k) sum += part[k][token].y * expf(part[k][token].x - from);
-        const float l = from + logf(sum);
+        const float2 a = part[0][token];
+        const float l = (a.x == -INFINITY ? 0.0f : a.x) + logf(a.y);
         const int t = rows[c];
         lse[t] = l;
         loss[t] = l - target[c];
@@ -250,11 +287,11 @@ bool sizes_ok(int hidden, int tokens, int vocab)
 // launches
 // ---------------------------------------------------------------------------
 
-template <typename T, Mode MODE, int BM, int BN, int WM, int WN>
+template <typename T, Mode MODE, int BM, int BN, int WM, int WN, bool ANY = false>
 int launch_tile(const ProductArgs &g, hipStream_t stream)
 {
-    auto kernel = product_kernel<T, MODE, BM, BN, WM, WN>;
-    constexpr int lds = Product<T, MODE, BM, BN, WM, WN>::kLds;
+    auto kernel = product_kernel<T, MODE, BM, BN, WM, WN, ANY>;
+    constexpr int lds = Product<T, MODE, BM, BN, WM, WN, ANY>::kLds;
     // LDS above the 64 KiB default needs an explicit opt-in, once per kernel and device.
     static std::atomic<unsigned> ready{0};
     int dev = 0;
@@ -276,13 +313,20 @@ int launch_tile(const ProductArgs &g, hipStream_t stream)
 }
 
 // The tile a product of M x N runs on.  N counts tokens in all products but GW.
-//  - up to 32 tokens: 128 x 32, of which four workgroups share a CU: the product is bound by the bytes of W then;
+//  - up to 32 tokens: 128 x 32, of which four workgroups share a CU: the product is bound by the bytes of W then, which
+//    may lie on any element (through registers) or on words (straight into LDS);
 //  - 256 x 256 where that fills most of the GPU's 256 CUs, with `splits` of k in GX;
 //  - else 128 x 128.
 enum Tile { NARROW, SMALL, LARGE };
-template <Mode MODE> Tile tile_for(int M, int N, int splits)
+constexpr int kNarrow = 32;
+#ifndef SHORT_T
+#define SHORT_T 512
+#endif
+constexpr int kShortTokens = SHORT_T;
+template <Mode MODE> Tile tile_for(int M, int N, int tokens, int splits)
 {
-    if (MODE != GW && N <= 32) return NARROW;
+    if (MODE != GW && N <= kNarrow) return NARROW;
+    if (MODE == GW && tokens <= kShortTokens) return SMALL;
     return (int64_t)((M + 255) / 256) * ((N + 255) / 256) * splits >= 200 ? LARGE : SMALL;
 }
 int tile_rows(Tile t) { return t == LARGE ? 256 : 128; }
@@ -353,22 +397,27 @@ template <typename T> Layout layout(int hidden, int tokens, int vocab, bool grad
     return l;
 }
 
-template <typename T, Mode MODE> int launch_product(const ProductArgs &g, hipStream_t stream)
+template <typename T, Mode MODE> int launch_product(const ProductArgs &g, bool words, hipStream_t stream)
 {
-    switch (tile_for<MODE>(g.M, g.N, MODE == GX ? g.splits : 1)) {
+    switch (tile_for<MODE>(g.M, g.N, MODE == GW ? g.K : g.N, MODE == GX ? g.splits : 1)) {
     case LARGE: return launch_tile<T, MODE, 256, 256, 2, 4>(g, stream);
     case SMALL: return launch_tile<T, MODE, 128, 128, 2, 2>(g, stream);
     default:
-        if constexpr (MODE != GW) return launch_tile<T, MODE, 128, 32, 4, 1>(g, stream);
+        if constexpr (MODE != GW) {
+            if constexpr (sizeof(T) == 2)
+                if (!words) return launch_tile<T, MODE, 128, 32, 4, 1, true>(g, stream);
+            return launch_tile<T, MODE, 128, 32, 4, 1>(g, stream);
+        }
         return ULMBLAS_GPU_BAD_ARGUMENT;        // GW has no narrow tile
     }
 }
 
-// Whether the product kernel can read W where it lies: rows that start on 4
-// bytes, and a tile's rows within 31 bits of each other.
-template <typename T> bool in_place(const T *W, int ldW)
+// Whether W's rows start on 4 bytes, as the copies straight into LDS need them, and whether the product kernel can read
+// W where it lies: then, or with the tile for few tokens; a tile's rows are within 31 bits of each other.
+template <typename T> bool on_words(const T *W, int ldW) { return ((uintptr_t)W & 3) == 0 && ldW * sizeof(T) % 4 == 0; }
+template <typename T> bool in_place(const T *W, int ldW, int tokens)
 {
-    return ((uintptr_t)W & 3) == 0 && ldW * sizeof(T) % 4 == 0 && (int64_t)ldW * (int64_t)sizeof(T) < (1 << 23);
+    return (on_words(W, ldW) || tokens <= kNarrow) && (int64_t)ldW * (int64_t)sizeof(T) < (1 << 23);
 }
 
 template <typename T>
@@ -379,6 +428,22 @@ int gather(const T *src, int64_t ld, int cols, const int *rows, const int *count
                        width);
     HIP_TRY(hipGetLastError());
     return ULMBLAS_GPU_OK;
+}
+
+// Which tokens count, and their rows of X side by side.
+constexpr int kFewTokens = 2048;        // up to here every workgroup counts for itself (a launch less: 4 us)
+template <typename T>
+int gather_tokens(const TokenArgs &t, const T *X, int64_t ldX, int hidden, T *Xc, int64_t width, hipStream_t stream)
+{
+    if (t.tokens > 0 && t.tokens <= kFewTokens) {
+        hipLaunchKernelGGL(token_gather_kernel<T>, dim3((unsigned)t.tokens), dim3(256), 0, stream, t, X, ldX, hidden, Xc,
+                           width);
+        HIP_TRY(hipGetLastError());
+        return ULMBLAS_GPU_OK;
+    }
+    hipLaunchKernelGGL(token_kernel, dim3(1), dim3(1024), 0, stream, t);
+    HIP_TRY(hipGetLastError());
+    return t.tokens > 0 ? gather<T>(X, ldX, hidden, t.rows, t.count, t.tokens, Xc, width, stream) : ULMBLAS_GPU_OK;
 }
 
 int bad(const char *text)
@@ -409,10 +474,8 @@ int xent_device(int hidden, int tokens, int vocab, float alpha, const T *W, int 
     t.count = part_of<int>(work, l.count);
     t.rows = part_of<int>(work, l.rows);
     t.label_c = part_of<int>(work, l.label);
-    hipLaunchKernelGGL(token_kernel, dim3(1), dim3(1024), 0, stream, t);
-    HIP_TRY(hipGetLastError());
     T *Xc = part_of<T>(work, l.x);
-    int rc = gather<T>(X, ldX, hidden, t.rows, t.count, tokens, Xc, l.hidden_p, stream);
+    int rc = gather_tokens<T>(t, X, ldX, hidden, Xc, l.hidden_p, stream);
     if (rc) return rc;
 
     ProductArgs g{};
@@ -426,7 +489,7 @@ int xent_device(int hidden, int tokens, int vocab, float alpha, const T *W, int 
     g.label = t.label_c;
     g.ldStats = l.tokens_p;
     g.target = part_of<float>(work, l.target);
-    const bool direct = in_place(W, ldW);
+    const bool direct = in_place(W, ldW, tokens), words = !direct || on_words(W, ldW);
     const int piece = direct ? vocab : l.piece;
     int tiles = 0;
     for (int v0 = 0; v0 < vocab; v0 += piece) {
@@ -445,12 +508,17 @@ int xent_device(int hidden, int tokens, int vocab, float alpha, const T *W, int 
             g.widthA = (int)l.hidden_p;
         }
         g.stats = part_of<float2>(work, l.stats) + (int64_t)tiles * l.tokens_p;
-        if ((rc = launch_product<T, STATS>(g, stream))) return rc;
-        const int bm = tile_rows(tile_for<STATS>(g.M, g.N, 1));
+        if ((rc = launch_product<T, STATS>(g, words, stream))) return rc;
+        const int bm = tile_rows(tile_for<STATS>(g.M, g.N, g.N, 1));
         tiles += (g.M + bm - 1) / bm;
     }
-    hipLaunchKernelGGL(loss_kernel<T>, dim3((unsigned)((tokens + 15) / 16)), dim3(256), 0, stream, tiles,
-                       part_of<float2>(work, l.stats), l.tokens_p, g.target, t.rows, t.count, loss, lse);
+    if (tokens <= 256) {
+        hipLaunchKernelGGL((loss_kernel<T, 0>), dim3((unsigned)tokens), dim3(256), 0, stream, tiles,
+                           part_of<float2>(work, l.stats), l.tokens_p, g.target, t.rows, t.count, loss, lse);
+    } else {
+        hipLaunchKernelGGL((loss_kernel<T, 4>), dim3((unsigned)((tokens + 15) / 16)), dim3(256), 0, stream, tiles,
+                           part_of<float2>(work, l.stats), l.tokens_p, g.target, t.rows, t.count, loss, lse);
+    }
     HIP_TRY(hipGetLastError());
     return ULMBLAS_GPU_OK;
 }
@@ -484,11 +552,9 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
     t.lse_c = part_of<float>(work, l.lse);
     t.both_c = part_of<float>(work, l.both);
     t.gloss_c = part_of<float>(work, l.gloss);
-    hipLaunchKernelGGL(token_kernel, dim3(1), dim3(1024), 0, stream, t);
-    HIP_TRY(hipGetLastError());
     T *Xc = part_of<T>(work, l.x), *P = part_of<T>(work, l.p);
-    int rc = ULMBLAS_GPU_OK;
-    if (tokens > 0 && (rc = gather<T>(X, ldX, hidden, t.rows, t.count, tokens, Xc, l.hidden_p, stream))) return rc;
+    int rc = gather_tokens<T>(t, X, ldX, hidden, Xc, l.hidden_p, stream);
+    if (rc) return rc;
     float *delta = part_of<float>(work, l.delta);
     int2 *member = part_of<int2>(work, l.member);
     int *rank = part_of<int>(work, l.rank), *bucket = part_of<int>(work, l.bucket);
@@ -500,7 +566,7 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
     // P: rows of blocks; all of them
     const int64_t row_x = l.hidden_p * (int64_t)sizeof(T), row_p = (int64_t)l.piece / kStep<T> * kBlockBytes;
     const int blocks_p = (int)(l.tokens_p / kBlockTokens * (l.piece / kStep<T>));
-    const bool direct = in_place(W, ldW);
+    const bool direct = in_place(W, ldW, tokens), words = !direct || on_words(W, ldW);
     for (int v0 = 0; v0 < vocab; v0 += l.piece) {
         const int vn = std::min(l.piece, vocab - v0);
         const T *Wv = W ? W + (int64_t)v0 * ldW : nullptr;
@@ -535,7 +601,7 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
             g.ldP = row_p;
             g.rank = rank;
             g.delta = delta;
-            if ((rc = launch_product<T, PROB>(g, stream))) return rc;
+            if ((rc = launch_product<T, PROB>(g, words, stream))) return rc;
         }
         if (gX && tokens > 0) {
             g.A = Wv;
@@ -552,7 +618,7 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
             g.splitStride = l.tokens_p * l.hidden_p;
             g.splits = l.splits;
             g.add = v0 > 0;
-            if ((rc = launch_product<T, GX>(g, stream))) return rc;
+            if ((rc = launch_product<T, GX>(g, words, stream))) return rc;
         }
         if (gW) {
             g.A = Xc;
@@ -571,7 +637,7 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
             g.out = gW + (int64_t)v0 * ldGW;
             g.ldD = ldGW;
             g.beta = beta;
-            if ((rc = launch_product<T, GW>(g, stream))) return rc;
+            if ((rc = launch_product<T, GW>(g, words, stream))) return rc;
         }
     }
     if (gX && tokens > 0) {

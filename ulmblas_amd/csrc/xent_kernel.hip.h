@@ -128,6 +128,11 @@ template <typename T, int CHUNKS> __device__ __forceinline__ int across_swizzle(
 // (rotating by the row itself costs every read twice its cycles).
 __device__ __forceinline__ int row_swizzle(int row) { return (row >> 1) & 7; }
 
+// 16 bytes at whatever address its elements have.
+template <typename T> struct AnyVector;
+template <> struct AnyVector<bf16_t> { typedef vint4 V __attribute__((aligned(2))); };
+template <> struct AnyVector<float> { typedef vint4 V __attribute__((aligned(4))); };
+
 // Brings R rows (or columns) of one operand for one step into LDS.
 template <typename T, int R, Lie LIE, int WAVES>
 struct Loader {
@@ -139,6 +144,7 @@ struct Loader {
     static constexpr int kStepsPerBlock = kBlockTokens / kStep<T>;
     static_assert(kCalls * WAVES * 1024 == kBytes, "the waves share the tile evenly");
 
+    vint4 held[kCalls];         // take() / put()
     uint64_t base;              // of the tile
     int64_t left;               // bytes of the operand from there on
     int64_t ld;
@@ -146,13 +152,15 @@ struct Loader {
     unsigned k_chunk;           // ALONG: byte inside the step this lane fetches in even calls (odd ones: 64 across)
     unsigned k_bytes;           // ALONG: bytes of a row that exist
 
+    // WORD: what the last row may be rounded up to (4 bytes for calls, nothing for take())
+    template <int64_t WORD = 4>
     __device__ void init(const void *p, int64_t ld_, int row0, int rows, int width, int wave, int lane)
     {
         ld = ld_;
         int64_t total, skip;
         if constexpr (LIE == ALONG || LIE == ACROSS) {
             // whole words: the buffer's range would cut off half of an odd row's last one
-            total = rows > 0 ? ((int64_t)(rows - 1) * ld + (int64_t)width * (int64_t)sizeof(T) + 3) & ~(int64_t)3 : 0;
+            total = rows > 0 ? ((int64_t)(rows - 1) * ld + (int64_t)width * (int64_t)sizeof(T) + WORD - 1) & -WORD : 0;
             skip = LIE == ALONG ? (int64_t)row0 * ld : (int64_t)row0 * (int64_t)sizeof(T);
         } else {
             total = (int64_t)width * kBlockBytes;
@@ -215,6 +223,37 @@ struct Loader {
                      : "s"(lds), "v"(off), "s"(rsrc)
                      : "memory");
     }
+
+    // The same through registers, for operands whose rows start on any element: all calls of step s, and their tile.
+    __device__ __forceinline__ void take(int s)
+    {
+        vint4 rsrc;
+        unsigned k_offset[2];
+        aim(s, rsrc, k_offset);
+        const int64_t skip = (int64_t)(((uint64_t)(uint32_t)rsrc[1] << 32 | (uint32_t)rsrc[0]) - (base & 0xffffffffffffull));
+        const unsigned have = (unsigned)rsrc[2];
+#pragma unroll
+        for (int c = 0; c < kCalls; ++c) {
+            const unsigned off = row_offset[c] + k_offset[c & 1];
+            const T *p = reinterpret_cast<const T *>(base + (uint64_t)skip + off);
+            held[c] = vint4{0, 0, 0, 0};
+            if (off < have && have - off >= 16) {
+                held[c] = *reinterpret_cast<const typename AnyVector<T>::V *>(p);
+            } else if (off < have) {            // the operand ends inside the chunk
+#pragma unroll
+                for (int e = 0; e < 16 / (int)sizeof(T); ++e) {
+                    if (e * sizeof(T) >= have - off) continue;
+                    if constexpr (sizeof(T) == 2) held[c][e >> 1] |= (int)((unsigned)p[e] << 16 * (e & 1));
+                    else held[c][e] = __float_as_int(p[e]);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void put(unsigned char *to, int wave, int lane) const
+    {
+#pragma unroll
+        for (int c = 0; c < kCalls; ++c) *reinterpret_cast<vint4 *>(to + (wave * kCalls + c) * 1024 + lane * 16) = held[c];
+    }
 };
 
 typedef __attribute__((address_space(3))) const unsigned char lds_byte;
@@ -264,17 +303,35 @@ template <typename T, int R, bool KC> struct Fragment {
     }
 };
 
-template <typename T>
-__device__ __forceinline__ vfloat4 multiply(vint4 a, vint4 b, vfloat4 c)
+// Which of a fragment's 16 bytes hold k that exist, `have` elements from its first on.
+template <typename T> __device__ __forceinline__ vint4 valid_k(int have)
+{
+    vint4 v;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if constexpr (sizeof(T) == 2) v[w] = have > 2 * w + 1 ? -1 : have > 2 * w ? 0xffff : 0;
+        else v[w] = have > w ? -1 : 0;
+    }
+    return v;
+}
+
+// One row of tiles: c[j] += a * b[j].  fp32 takes the four k of a fragment one
+// after the other for all tiles, so that no matrix instruction waits for the
+// one before it.
+template <typename T, int TN>
+__device__ __forceinline__ void multiply(vint4 a, const vint4 (&b)[TN], vfloat4 (&c)[TN])
 {
     if constexpr (sizeof(T) == 2) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vbf8, a), __builtin_bit_cast(vbf8, b), c, 0,
-                                                       0, 0);
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+            c[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vbf8, a), __builtin_bit_cast(vbf8, b[j]),
+                                                           c[j], 0, 0, 0);
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__int_as_float(a[j]), __int_as_float(b[j]), c, 0, 0, 0);
-        return c;
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+                c[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__int_as_float(a[e]), __int_as_float(b[j][e]), c[j], 0, 0, 0);
     }
 }
 
@@ -316,7 +373,7 @@ __device__ __forceinline__ bool tile_of(int id, int tilesM, int tilesN, int &tm,
     return true;
 }
 
-template <typename T, Mode MODE, int BM, int BN, int WM, int WN>
+template <typename T, Mode MODE, int BM, int BN, int WM, int WN, bool ANY>
 struct Product {
     static constexpr int kWaves = WM * WN;
     static constexpr int kThreads = kWaves * 64;
@@ -340,11 +397,6 @@ template <int BM> __device__ __forceinline__ int staged_at(int row, int col)
     constexpr int kChunks = BM / 8;
     return row * (BM * 2) + (((col >> 3) ^ (row & (kChunks - 1))) << 4) + (col & 7) * 2;
 }
-
-// 16 bytes at whatever address its elements have.
-template <typename T> struct AnyVector;
-template <> struct AnyVector<bf16_t> { typedef vint4 V __attribute__((aligned(2))); };
-template <> struct AnyVector<float> { typedef vint4 V __attribute__((aligned(4))); };
 
 // Writes the staged tile out, whole rows at a time: rows x cols of it.
 template <int BM, int THREADS>
@@ -428,8 +480,8 @@ __device__ __forceinline__ void add_label_remainders(const ProductArgs &g, int m
     }
 }
 
-template <typename T, Mode MODE, int BM, int BN, int WM, int WN>
-__device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
+template <typename T, Mode MODE, int BM, int BN, int WM, int WN, bool ANY>
+__device__ void Product<T, MODE, BM, BN, WM, WN, ANY>::run(const ProductArgs &g)
 {
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds_raw[];
     lds_byte *lds = (lds_byte *)lds_raw;
@@ -455,8 +507,8 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
     LoadA la;
     LoadB lb;
     // ALONG: rows of D's side, of `width` elements; ACROSS: rows of k
-    la.init(g.A, g.ldA, m0, A_KC ? g.M : K, g.widthA, wave, lane);
-    lb.init(g.B, g.ldB, n0, B_KC ? boundN : K, g.widthB, wave, lane);
+    la.template init<(ANY ? 1 : 4)>(g.A, g.ldA, m0, A_KC ? g.M : K, g.widthA, wave, lane);
+    lb.template init<(ANY ? 1 : 4)>(g.B, g.ldB, n0, B_KC ? boundN : K, g.widthB, wave, lane);
 
     vfloat4 acc[TM][TN];
 #pragma unroll
@@ -466,6 +518,36 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[i][j][r] = 0.0f;
 
+    if constexpr (ANY) {
+        // Through registers: the next step is on its way while this one is multiplied; several workgroups share a CU.
+        const unsigned lane_a = Fragment<T, BM, A_KC>::base(wm * TM * 16, lane);
+        const unsigned lane_b = Fragment<T, BN, B_KC>::base(wn * TN * 16, lane) + BM * kStepBytes;
+        if (s0 < s1) {
+            la.take(s0);
+            lb.take(s0);
+        }
+        for (int s = s0; s < s1; ++s) {
+            const unsigned half = ((s - s0) & 1) * kStage;
+            la.put(lds_raw + half, wave, lane);
+            lb.put(lds_raw + half + BM * kStepBytes, wave, lane);
+            __syncthreads();        // also: nobody reads the other half any more
+            if (s + 1 < s1) {
+                la.take(s + 1);
+                lb.take(s + 1);
+            }
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                vint4 b[TN];
+#pragma unroll
+                for (int j = 0; j < TN; ++j) b[j] = Fragment<T, BN, B_KC>::read(lds, lane_b + half, j, kk);
+                vint4 valid = {-1, -1, -1, -1};
+                if (LIE_A == ALONG && s + 1 == s1) valid = valid_k<T>(K - s * kStep<T> - (4 * kk + (lane >> 4)) * (16 / (int)sizeof(T)));
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+                    multiply<T>(Fragment<T, BM, A_KC>::read(lds, lane_a + half, i, kk) & valid, b, acc[i]);
+            }
+        }
+    } else
     // Two halves of LDS, a step each; a step is two halves of k, and the TM rows
     // of MFMA tiles of one half are a group each.  The fragment of A is read
     // three groups ahead into a ring of four, those of B for one half of k while
@@ -508,8 +590,7 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
         auto group = [&](int g, bool last) {
             vint4 x = a[g % RING];
             if (LIE_A == ALONG && last) x &= valid[g / TM];
-#pragma unroll
-            for (int j = 0; j < TN; ++j) acc[g % TM][j] = multiply<T>(x, b[g / TM][j], acc[g % TM][j]);
+            multiply<T>(x, b[g / TM], acc[g % TM]);
         };
         aim(s0, 0);
 #pragma unroll
@@ -563,12 +644,7 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
         if constexpr (LIE_A == ALONG) {
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
-                const int have = K - (s1 - 1) * kStep<T> - (4 * kk + (lane >> 4)) * (16 / (int)sizeof(T));
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    if constexpr (sizeof(T) == 2) valid[kk][w] = have > 2 * w + 1 ? -1 : have > 2 * w ? 0xffff : 0;
-                    else valid[kk][w] = have > w ? -1 : 0;
-                }
+                valid[kk] = valid_k<T>(K - (s1 - 1) * kStep<T> - (4 * kk + (lane >> 4)) * (16 / (int)sizeof(T)));
             }
         }
         most(true);
@@ -759,11 +835,11 @@ __device__ void Product<T, MODE, BM, BN, WM, WN>::run(const ProductArgs &g)
     }
 }
 
-template <typename T, Mode MODE, int BM, int BN, int WM, int WN>
+template <typename T, Mode MODE, int BM, int BN, int WM, int WN, bool ANY>
 __global__ void __launch_bounds__(WM *WN * 64, 2)
 product_kernel(ProductArgs g)
 {
-    Product<T, MODE, BM, BN, WM, WN>::run(g);
+    Product<T, MODE, BM, BN, WM, WN, ANY>::run(g);
 }
 
 }  // namespace xent
