@@ -235,8 +235,8 @@ loss_kernel(int tiles, const float2 *__restrict__ stats, int64_t ld, const float
 // took from P at the label), or zeros.  Four elements a thread.
 template <typename T>
 __global__ void __launch_bounds__(256)
-gx_kernel(int hidden, const int *__restrict__ place, const float *__restrict__ part, int64_t ld, int64_t stride,
-          int splits, const float *__restrict__ delta, const int *__restrict__ rank, const int *__restrict__ label,
+gx_kernel(int hidden, const int *__restrict__ place, const int *__restrict__ count, int rows, int columns, int groups,
+          int steps, const float *__restrict__ part, int64_t ld, const float *__restrict__ delta, const int *__restrict__ rank, const int *__restrict__ label,
           const T *__restrict__ W, int64_t ldw, T *gx, int64_t ldgx)
 {
     const int t = blockIdx.x, c = place[t], h = (int)(blockIdx.y * 256 + threadIdx.x) * 4;
@@ -250,6 +250,9 @@ gx_kernel(int hidden, const int *__restrict__ place, const float *__restrict__ p
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = e < n ? d * to_float(w[e]) : 0.0f;
         }
+        const int live = *count, tiles = (hidden + rows - 1) / rows * ((live + columns - 1) / columns);
+        const int splits = splits_of(groups, tiles, steps);
+        const int64_t stride = live * ld;
         const float *p = part + c * ld + h;
         int s = 0;
         for (; s + 4 <= splits; s += 4) {
@@ -287,11 +290,11 @@ bool sizes_ok(int hidden, int tokens, int vocab)
 // launches
 // ---------------------------------------------------------------------------
 
-template <typename T, Mode MODE, int BM, int BN, int WM, int WN, bool ANY = false>
+template <typename T, Mode MODE, int BM, int BN, int WM, int WN, int BUFFERS = 2, bool ANY = false>
 int launch_tile(const ProductArgs &g, hipStream_t stream)
 {
-    auto kernel = product_kernel<T, MODE, BM, BN, WM, WN, ANY>;
-    constexpr int lds = Product<T, MODE, BM, BN, WM, WN, ANY>::kLds;
+    auto kernel = product_kernel<T, MODE, BM, BN, WM, WN, BUFFERS, ANY>;
+    constexpr int lds = Product<T, MODE, BM, BN, WM, WN, BUFFERS, ANY>::kLds;
     // LDS above the 64 KiB default needs an explicit opt-in, once per kernel and device.
     static std::atomic<unsigned> ready{0};
     int dev = 0;
@@ -306,46 +309,89 @@ int launch_tile(const ProductArgs &g, hipStream_t stream)
         g_last_error = "too many tiles for one launch";
         return ULMBLAS_GPU_BAD_ARGUMENT;
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, MODE == GX ? (unsigned)g.splits : 1u), dim3(WM * WN * 64), lds,
-                       stream, g);
+    // a single step of k needs one tile of LDS, and what the result is staged in
+    constexpr int one = std::max(Product<T, MODE, BM, BN, WM, WN, BUFFERS, ANY>::kStage, BM * BN * 2);
+    const bool single = BUFFERS == 2 && !ANY && MODE == GW && g.K <= kStep<T>;
+    const unsigned grid = (unsigned)(MODE == GX ? std::max<int64_t>(tiles, g.groups) : tiles);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(WM * WN * 64), single ? one : lds, stream, g);
     HIP_TRY(hipGetLastError());
     return ULMBLAS_GPU_OK;
 }
 
-// The tile a product of M x N runs on.  N counts tokens in all products but GW.
-//  - up to 32 tokens: 128 x 32, of which four workgroups share a CU: the product is bound by the bytes of W then, which
-//    may lie on any element (through registers) or on words (straight into LDS);
-//  - 256 x 256 where that fills most of the GPU's 256 CUs, with `splits` of k in GX;
-//  - else 128 x 128.
-enum Tile { NARROW, SMALL, LARGE };
+// The tile a product runs on: the one with the least estimated time.  The CUs
+// share the tiles, so the CU with the most of them counts:
+//
+//   time = ceil(tiles / 256) * (rows * columns * K / (rate * efficiency) + overhead)
+//
+// in microseconds, with the rate of the 256 x 256 tile on large products (bf16
+// 1250 TFLOP/s, fp32 122) and what the others reached on the same ones (tokens
+// 2048, hidden 1024; bf16 vocabulary 32768, fp32 16384):
+//
+//                 logits                GX                 overhead (beginning, end; writing for GW)
+//   256 x 256     127 us / 566 us       145 us / 562 us    8.5   12
+//   128 x 128     151    / 595          135    / 574       1.5    3.2 (2.2 with a single step of k)
+//   128 x 64      184    / 605          181    / 596       1.5
+//   128 x 32             / 666                 / 650       1.5
+//
+// The tile for 32 columns is also the one that takes W on any element, so bf16
+// keeps to it there; wider bf16 products would write P past its rows with it.
+// GX may cut k, so that any tile fills the GPU: it counts whole rounds.
+struct Tile {
+    int rows, columns;
+};
+constexpr Tile kTiles[] = {{256, 256}, {128, 128}, {128, 64}, {128, 32}};
 constexpr int kNarrow = 32;
-#ifndef SHORT_T
-#define SHORT_T 512
-#endif
-constexpr int kShortTokens = SHORT_T;
-template <Mode MODE> Tile tile_for(int M, int N, int tokens, int splits)
-{
-    if (MODE != GW && N <= kNarrow) return NARROW;
-    if (MODE == GW && tokens <= kShortTokens) return SMALL;
-    return (int64_t)((M + 255) / 256) * ((N + 255) / 256) * splits >= 200 ? LARGE : SMALL;
-}
-int tile_rows(Tile t) { return t == LARGE ? 256 : 128; }
+constexpr int kGroups = 512;            // workgroups GX is spread over: two rounds, so that some tokens may be missing
 
-// Into how many parts k of GX is cut: two rounds of workgroups if every token
-// has a target, as much as it takes with the small tile if there are few tiles.
-int splits_of_gx(int hidden, int tokens, int piece)
+template <typename T, Mode MODE> Tile choose(int M, int N, int K)
 {
-    const int64_t large = ((hidden + 255) / 256) * (int64_t)((tokens + 255) / 256);
-    const int64_t small = ((hidden + 127) / 128) * (int64_t)((tokens + 127) / 128);
-    const int64_t want = large >= 16 ? 512 / large : 512 / small;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 64), piece / 512));
+    constexpr bool half = sizeof(T) == 2;
+    if (half && MODE != GW && N <= kNarrow) return kTiles[3];
+    constexpr double rate = half ? 2.44e6 : 0.238e6;            // products and sums a CU and microsecond
+    constexpr double efficiency[4] = {1.0, half ? 0.83 : 0.95, half ? 0.69 : 0.93, 0.84};
+    int best = 0;
+    double least = 0.0;
+    for (int t = 0; t < 4; ++t) {
+        if ((MODE == GW && t > 1) || (half && t == 3)) continue;
+        const double tiles = (double)((M + kTiles[t].rows - 1) / kTiles[t].rows) *
+                             ((N + kTiles[t].columns - 1) / kTiles[t].columns);
+        const double rounds = MODE == GX ? std::max(1.0, tiles / 256) : std::ceil(tiles / 256);
+        double k = K, overhead = t == 0 ? 8.5 : 1.5;
+        if (MODE == GX) k = k * std::min(1.0, std::max(tiles / 256, 8.0 * kStep<T> / std::max(K, 1)));
+        if (MODE == GW) overhead = t == 0 ? 12.0 : K <= kStep<T> ? 2.2 : 3.2;
+        const double time = rounds * (kTiles[t].rows * kTiles[t].columns * k / (rate * efficiency[t]) + overhead);
+        if (t == 0 || time < least) {
+            best = t;
+            least = time;
+        }
+    }
+    return kTiles[best];
+}
+
+template <typename T, Mode MODE> int launch_product(const ProductArgs &g, Tile tile, bool words, hipStream_t stream)
+{
+    const int64_t groups = (int64_t)((g.M + tile.rows - 1) / tile.rows) * ((g.N + tile.columns - 1) / tile.columns);
+    if (tile.rows == 256) return launch_tile<T, MODE, 256, 256, 2, 4>(g, stream);
+    if constexpr (MODE == GW) {
+        return launch_tile<T, MODE, 128, 128, 2, 2>(g, stream);
+    } else {
+        if (tile.columns == 32) {
+            if constexpr (sizeof(T) == 2)
+                if (!words) return launch_tile<T, MODE, 128, 32, 4, 1, 2, true>(g, stream);
+            return launch_tile<T, MODE, 128, 32, 4, 1, 4>(g, stream);
+        }
+        if (tile.columns == 64) return launch_tile<T, MODE, 128, 64, 2, 2, 3>(g, stream);
+        // alone on its CU a workgroup keeps more steps open
+        if (MODE != GX && groups <= 256) return launch_tile<T, MODE, 128, 128, 2, 2, 4>(g, stream);
+        return launch_tile<T, MODE, 128, 128, 2, 2>(g, stream);
+    }
 }
 
 // What the workspace holds and where; every part starts on 256 bytes.
 struct Layout {
     int64_t tokens_p, hidden_p;         // rounded up: rows of compact copies, elements of their rows
     int piece;                          // vocabulary rows at a time (gradient: of P; packing: of W)
-    int splits;                         // partial sums of gX
+    Tile gx;                            // tile of GX
     int64_t rows, label, place, lse, both, gloss, delta, target, bucket, member, rank, count, x, w, stats, p, part, bytes;
 };
 
@@ -361,10 +407,7 @@ template <typename T> Layout layout(int hidden, int tokens, int vocab, bool grad
     piece = std::min<int64_t>(piece, 1 << 19);
     if (g_piece_rows.load() > 0) piece = std::min<int64_t>(piece, round_up(g_piece_rows.load(), 256));
     l.piece = (int)std::min<int64_t>(piece, round_up(vocab, 256));
-    l.splits = 1;
-    if (grad) {
-        l.splits = splits_of_gx(hidden, std::max(tokens, 1), l.piece);
-    }
+    l.gx = choose<T, GX>(hidden, std::max(tokens, 1), l.piece);
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t here = at;
@@ -391,25 +434,11 @@ template <typename T> Layout layout(int hidden, int tokens, int vocab, bool grad
         l.stats = take((round_up(vocab, 256) / 128) * l.tokens_p * 8);
     } else {
         l.p = take(l.tokens_p * l.piece * (int64_t)sizeof(T));
-        l.part = take((int64_t)l.splits * l.tokens_p * l.hidden_p * 4);
+        // as many splits as fill kGroups workgroups with tiles, or one
+        l.part = take(std::max((int64_t)kGroups * l.gx.rows * l.gx.columns, l.tokens_p * l.hidden_p) * 4);
     }
     l.bytes = at;
     return l;
-}
-
-template <typename T, Mode MODE> int launch_product(const ProductArgs &g, bool words, hipStream_t stream)
-{
-    switch (tile_for<MODE>(g.M, g.N, MODE == GW ? g.K : g.N, MODE == GX ? g.splits : 1)) {
-    case LARGE: return launch_tile<T, MODE, 256, 256, 2, 4>(g, stream);
-    case SMALL: return launch_tile<T, MODE, 128, 128, 2, 2>(g, stream);
-    default:
-        if constexpr (MODE != GW) {
-            if constexpr (sizeof(T) == 2)
-                if (!words) return launch_tile<T, MODE, 128, 32, 4, 1, true>(g, stream);
-            return launch_tile<T, MODE, 128, 32, 4, 1>(g, stream);
-        }
-        return ULMBLAS_GPU_BAD_ARGUMENT;        // GW has no narrow tile
-    }
 }
 
 // Whether W's rows start on 4 bytes, as the copies straight into LDS need them, and whether the product kernel can read
@@ -508,9 +537,9 @@ int xent_device(int hidden, int tokens, int vocab, float alpha, const T *W, int 
             g.widthA = (int)l.hidden_p;
         }
         g.stats = part_of<float2>(work, l.stats) + (int64_t)tiles * l.tokens_p;
-        if ((rc = launch_product<T, STATS>(g, words, stream))) return rc;
-        const int bm = tile_rows(tile_for<STATS>(g.M, g.N, g.N, 1));
-        tiles += (g.M + bm - 1) / bm;
+        const Tile tile = choose<T, STATS>(g.M, g.N, g.K);
+        if ((rc = launch_product<T, STATS>(g, tile, words, stream))) return rc;
+        tiles += (g.M + tile.rows - 1) / tile.rows;
     }
     if (tokens <= 256) {
         hipLaunchKernelGGL((loss_kernel<T, 0>), dim3((unsigned)tokens), dim3(256), 0, stream, tiles,
@@ -601,7 +630,7 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
             g.ldP = row_p;
             g.rank = rank;
             g.delta = delta;
-            if ((rc = launch_product<T, PROB>(g, words, stream))) return rc;
+            if ((rc = launch_product<T, PROB>(g, choose<T, PROB>(g.M, g.N, g.K), words, stream))) return rc;
         }
         if (gX && tokens > 0) {
             g.A = Wv;
@@ -615,10 +644,10 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
             g.K = vn;
             g.part = part_of<float>(work, l.part);
             g.ldD = l.hidden_p;
-            g.splitStride = l.tokens_p * l.hidden_p;
-            g.splits = l.splits;
+            g.groups = kGroups;
+            g.steps = (l.piece + kStep<T> - 1) / kStep<T>;
             g.add = v0 > 0;
-            if ((rc = launch_product<T, GX>(g, words, stream))) return rc;
+            if ((rc = launch_product<T, GX>(g, l.gx, words, stream))) return rc;
         }
         if (gW) {
             g.A = Xc;
@@ -637,12 +666,13 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
             g.out = gW + (int64_t)v0 * ldGW;
             g.ldD = ldGW;
             g.beta = beta;
-            if ((rc = launch_product<T, GW>(g, words, stream))) return rc;
+            if ((rc = launch_product<T, GW>(g, choose<T, GW>(g.M, g.N, g.K), words, stream))) return rc;
         }
     }
     if (gX && tokens > 0) {
         hipLaunchKernelGGL(gx_kernel<T>, dim3((unsigned)tokens, (unsigned)((hidden + 1023) / 1024)), dim3(256), 0, stream, hidden, t.place,
-                           part_of<float>(work, l.part), l.hidden_p, l.tokens_p * l.hidden_p, l.splits, delta, rank,
+                           t.count, l.gx.rows, l.gx.columns, kGroups, (l.piece + kStep<T> - 1) / kStep<T>,
+                           part_of<float>(work, l.part), l.hidden_p, delta, rank,
                            t.label_c, W, (int64_t)ldW, gX,
                            (int64_t)ldGX);
         HIP_TRY(hipGetLastError());

@@ -103,10 +103,10 @@ struct ProductArgs {
     int64_t ldP;                // bytes from one row of blocks to the next
     const int *rank;            // per token: its place in `member`
     float *delta;               // per place there: what rounding took from P at the label (PROB writes, GW reads)
-    // GX: partial sums of the splits, each [token][ldD]
+    // GX: partial sums of the splits, each [token][ldD], one after the other as long as `count` makes them
     float *part;
-    int64_t ldD, splitStride;
-    int splits, add;
+    int64_t ldD;                // elements; GW: of out
+    int groups, steps, add;     // workgroups to spread over, steps of k of a whole piece; whether there are sums to add to
     // GW
     void *out;
     float beta;
@@ -188,7 +188,7 @@ struct Loader {
     }
 
     // step s of the k loop: the buffer and the offsets its calls use
-    __device__ __forceinline__ void aim(int s, vint4 &rsrc, unsigned (&k_offset)[2]) const
+    __device__ __forceinline__ void aim(int s, int end, vint4 &rsrc, unsigned (&k_offset)[2]) const
     {
         int64_t skip = 0;
         k_offset[0] = k_offset[1] = 0;
@@ -206,7 +206,7 @@ struct Loader {
         }
         const uint64_t at = base + (uint64_t)skip;
         int64_t have = left - skip;
-        have = have < 0 ? 0 : (have > 0x7fffffff ? 0x7fffffff : have);
+        have = have < 0 || s >= end ? 0 : (have > 0x7fffffff ? 0x7fffffff : have);
         rsrc[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)at);
         rsrc[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32) & 0xffff);
         rsrc[2] = __builtin_amdgcn_readfirstlane((int)have);
@@ -229,7 +229,7 @@ struct Loader {
     {
         vint4 rsrc;
         unsigned k_offset[2];
-        aim(s, rsrc, k_offset);
+        aim(s, s + 1, rsrc, k_offset);
         const int64_t skip = (int64_t)(((uint64_t)(uint32_t)rsrc[1] << 32 | (uint32_t)rsrc[0]) - (base & 0xffffffffffffull));
         const unsigned have = (unsigned)rsrc[2];
 #pragma unroll
@@ -348,32 +348,41 @@ template <typename T> __device__ __forceinline__ float exponential(float x)
     else return expf(x);
 }
 
-// Everything this wave has asked for has arrived, and every wave of the
-// workgroup says so.
-__device__ __forceinline__ void wait_and_meet()
+// All but the OPEN latest fetches of this wave have arrived, it has read all it
+// asked LDS for, and every wave of the workgroup says so.
+template <int OPEN = 0> __device__ __forceinline__ void wait_and_meet()
 {
-    __builtin_amdgcn_s_waitcnt(0x0070);         // tells the compiler; the next line is what counts
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    static_assert(OPEN < 64, "six bits");
+    __builtin_amdgcn_s_waitcnt(0x0070 | (OPEN & 15) | (OPEN >> 4) << 14);       // tells the compiler; the next line is what counts
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(OPEN) : "memory");
+}
+
+// Into how many parts GX cuts its k: what fills `groups` workgroups with the
+// tokens that count, parts of at least 8 steps.
+constexpr int kMaxSplits = 64;
+__device__ __forceinline__ int splits_of(int groups, int tiles, int steps)
+{
+    int n = tiles > 0 ? groups / tiles : 1;
+    n = n < steps / 8 ? n : steps / 8;
+    return n < 1 ? 1 : (n > kMaxSplits ? kMaxSplits : n);
 }
 
 // Which tile of D workgroup `id` computes.  Workgroups go round the 8 XCDs;
 // each XCD takes a run of consecutive tiles, ordered in bands of 8 columns, so
 // that the 32 tiles its CUs work on at a time are 8 x 4 and share operands in
 // its L2.
-__device__ __forceinline__ bool tile_of(int id, int tilesM, int tilesN, int &tm, int &tn)
+__device__ __forceinline__ void tile_of(int id, int tilesM, int tilesN, int &tm, int &tn)
 {
     const int tiles = tilesM * tilesN;
-    if (id >= tiles) return false;
     const int per = tiles / 8, extra = tiles % 8, x = id % 8;
     id = x * per + (x < extra ? x : extra) + id / 8;
     const int band = id / (8 * tilesM), at = id % (8 * tilesM);
     const int width = tilesN - band * 8 < 8 ? tilesN - band * 8 : 8;
     tn = band * 8 + at % width;
     tm = at / width;
-    return true;
 }
 
-template <typename T, Mode MODE, int BM, int BN, int WM, int WN, bool ANY>
+template <typename T, Mode MODE, int BM, int BN, int WM, int WN, int BUFFERS, bool ANY>
 struct Product {
     static constexpr int kWaves = WM * WN;
     static constexpr int kThreads = kWaves * 64;
@@ -382,7 +391,8 @@ struct Product {
     static constexpr Lie LIE_B = MODE == GX ? P_ALONG : MODE == GW ? P_ACROSS : ALONG;
     static constexpr bool A_KC = k_contiguous(LIE_A), B_KC = k_contiguous(LIE_B);
     static constexpr int kStage = (BM + BN) * kStepBytes;
-    static constexpr int kLds = 2 * kStage;
+    static constexpr int kLds = BUFFERS * kStage;
+    static_assert(!ANY || BUFFERS == 2, "through registers: two halves");
     using LoadA = Loader<T, BM, LIE_A, kWaves>;
     using LoadB = Loader<T, BN, LIE_B, kWaves>;
 
@@ -480,8 +490,8 @@ __device__ __forceinline__ void add_label_remainders(const ProductArgs &g, int m
     }
 }
 
-template <typename T, Mode MODE, int BM, int BN, int WM, int WN, bool ANY>
-__device__ void Product<T, MODE, BM, BN, WM, WN, ANY>::run(const ProductArgs &g)
+template <typename T, Mode MODE, int BM, int BN, int WM, int WN, int BUFFERS, bool ANY>
+__device__ void Product<T, MODE, BM, BN, WM, WN, BUFFERS, ANY>::run(const ProductArgs &g)
 {
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds_raw[];
     lds_byte *lds = (lds_byte *)lds_raw;
@@ -493,16 +503,22 @@ __device__ void Product<T, MODE, BM, BN, WM, WN, ANY>::run(const ProductArgs &g)
     // Columns past the tokens that count have no tile.
     const int live = __builtin_amdgcn_readfirstlane(*g.count);
     const int boundN = MODE == GW ? g.N : (live < g.N ? live : g.N);
-    int tm, tn;
-    if (!tile_of((int)blockIdx.x, (g.M + BM - 1) / BM, (boundN + BN - 1) / BN, tm, tn)) return;
-    const int m0 = tm * BM, n0 = tn * BN;
     const int K = MODE == GW ? (live < g.K ? live : g.K) : g.K;
-    int s0 = 0, s1 = (K + kStep<T> - 1) / kStep<T>;
+    const int tilesM = (g.M + BM - 1) / BM, tilesN = (boundN + BN - 1) / BN, tiles = tilesM * tilesN;
+    int s0 = 0, s1 = (K + kStep<T> - 1) / kStep<T>, split = 0, id = blockIdx.x;
     if constexpr (MODE == GX) {
-        const int steps = s1, z = blockIdx.y;
-        s0 = (int)((int64_t)steps * z / g.splits);
-        s1 = (int)((int64_t)steps * (z + 1) / g.splits);
+        const int splits = splits_of(g.groups, tiles, g.steps), steps = s1;
+        if (id >= tiles * splits) return;
+        split = id / tiles;
+        id -= split * tiles;
+        s0 = (int)((int64_t)steps * split / splits);
+        s1 = (int)((int64_t)steps * (split + 1) / splits);
+    } else if (id >= tiles) {
+        return;
     }
+    int tm, tn;
+    tile_of(id, tilesM, tilesN, tm, tn);
+    const int m0 = tm * BM, n0 = tn * BN;
 
     LoadA la;
     LoadB lb;
@@ -548,13 +564,13 @@ __device__ void Product<T, MODE, BM, BN, WM, WN, ANY>::run(const ProductArgs &g)
             }
         }
     } else
-    // Two halves of LDS, a step each; a step is two halves of k, and the TM rows
-    // of MFMA tiles of one half are a group each.  The fragment of A is read
+    // BUFFERS tiles in LDS, a step each; a step is two halves of k, and the TM
+    // rows of MFMA tiles of one half are a group each.  The fragment of A is read
     // three groups ahead into a ring of four, those of B for one half of k while
     // the other half is multiplied.  The step changes three groups before its
-    // end: all its fragments are in registers by then, so the half just read can
-    // be refilled for the step after next, and the matrix cores have work while
-    // the waves meet and the next step's first fragments come out of LDS.
+    // end: all its fragments are in registers by then, so the tile just read can
+    // be refilled, and the matrix cores have work while the waves meet and the
+    // next step's first fragments come out of LDS.
     if (s0 < s1) {
         constexpr int RING = 4, AHEAD = 3, GROUPS = 2 * TM, LAST = GROUPS - AHEAD, SPREAD = TM < LAST ? TM : LAST;
         static_assert(GROUPS % RING == 0, "the ring closes with the step");
@@ -577,8 +593,8 @@ __device__ void Product<T, MODE, BM, BN, WM, WN, ANY>::run(const ProductArgs &g)
         unsigned ka[2], kb[2], to = 0;
         constexpr int kCalls = LoadA::kCalls + LoadB::kCalls;
         auto aim = [&](int s, unsigned at) {
-            la.aim(s, ra, ka);
-            lb.aim(s, rb, kb);
+            la.aim(s, s1, ra, ka);
+            lb.aim(s, s1, rb, kb);
             to = lds0 + at;
         };
         auto call = [&](int c) {
@@ -592,14 +608,23 @@ __device__ void Product<T, MODE, BM, BN, WM, WN, ANY>::run(const ProductArgs &g)
             if (LIE_A == ALONG && last) x &= valid[g / TM];
             multiply<T>(x, b[g / TM], acc[g % TM]);
         };
+        // Steps past the end are asked for too where more than two tiles are open (they bring zeros), so that what
+        // is open is the same number of calls in every step.
+        constexpr int kOpen = (BUFFERS - 2) * kCalls;
         aim(s0, 0);
 #pragma unroll
         for (int c = 0; c < kCalls; ++c) call(c);
         if constexpr (MODE == GW && sizeof(T) == 2)
             add_label_remainders<T, BM, BN, WM, WN>(g, m0, n0, wm, wn, lane, acc);
-        wait_and_meet();
-        if (s0 + 1 < s1) {
-            aim(s0 + 1, kStage);
+#pragma unroll
+        for (int x = 1; x + 1 < BUFFERS; ++x) {
+            aim(s0 + x, x * kStage);
+#pragma unroll
+            for (int c = 0; c < kCalls; ++c) call(c);
+        }
+        wait_and_meet<kOpen>();
+        if (BUFFERS > 2 || s0 + 1 < s1) {
+            aim(s0 + BUFFERS - 1, (BUFFERS - 1) * kStage);
 #pragma unroll
             for (int c = 0; c < kCalls; ++c) call(c);
         }
@@ -622,10 +647,10 @@ __device__ void Product<T, MODE, BM, BN, WM, WN, ANY>::run(const ProductArgs &g)
         };
         for (int s = s0; s + 1 < s1; ++s) {
             most(false);
-            wait_and_meet();
-            const bool more = s + 2 < s1;
-            if (more) aim(s + 2, now);
-            now = kStage - now;
+            wait_and_meet<kOpen>();
+            const bool more = BUFFERS > 2 || s + 2 < s1;
+            if (more) aim(s + BUFFERS, now);
+            now = now + kStage == kLds ? 0 : now + kStage;
             read_from(now);
 #pragma unroll
             for (int g = LAST; g < GROUPS; ++g) {
@@ -650,6 +675,7 @@ __device__ void Product<T, MODE, BM, BN, WM, WN, ANY>::run(const ProductArgs &g)
         most(true);
 #pragma unroll
         for (int g = LAST; g < GROUPS; ++g) group(g, true);
+        if constexpr (BUFFERS > 2) wait_and_meet();         // nothing may be on its way into LDS when the workgroup ends
     }
 
     const int mw = m0 + wm * TM * 16 + (lane >> 4) * 4, nw = n0 + wn * TN * 16 + (lane & 15);
@@ -780,7 +806,7 @@ __device__ void Product<T, MODE, BM, BN, WM, WN, ANY>::run(const ProductArgs &g)
             }
         }
     } else if constexpr (MODE == GX) {
-        float *part = g.part + (int64_t)blockIdx.y * g.splitStride;
+        float *part = g.part + (int64_t)split * boundN * g.ldD;
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
             const int n = nw + j * 16;
@@ -835,11 +861,11 @@ __device__ void Product<T, MODE, BM, BN, WM, WN, ANY>::run(const ProductArgs &g)
     }
 }
 
-template <typename T, Mode MODE, int BM, int BN, int WM, int WN, bool ANY>
-__global__ void __launch_bounds__(WM *WN * 64, 2)
+template <typename T, Mode MODE, int BM, int BN, int WM, int WN, int BUFFERS, bool ANY>
+__global__ void __launch_bounds__(WM *WN * 64, MODE == GW && WM * WN == 4 ? 3 : 2)
 product_kernel(ProductArgs g)
 {
-    Product<T, MODE, BM, BN, WM, WN, ANY>::run(g);
+    Product<T, MODE, BM, BN, WM, WN, BUFFERS, ANY>::run(g);
 }
 
 }  // namespace xent
