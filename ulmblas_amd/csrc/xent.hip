@@ -240,6 +240,8 @@ gx_kernel(int hidden, const int *__restrict__ place, const int *__restrict__ cou
           const T *__restrict__ W, int64_t ldw, T *gx, int64_t ldgx)
 {
     const int t = blockIdx.x, c = place[t], h = (int)(blockIdx.y * 256 + threadIdx.x) * 4;
+    const int live = *count, tiles = (hidden + rows - 1) / rows * ((live + columns - 1) / columns);
+    const int splits = splits_of(groups, tiles, steps, live, hidden);
     if (h >= hidden) return;
     const int n = hidden - h < 4 ? hidden - h : 4;
     vfloat4 v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -250,8 +252,6 @@ gx_kernel(int hidden, const int *__restrict__ place, const int *__restrict__ cou
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = e < n ? d * to_float(w[e]) : 0.0f;
         }
-        const int live = *count, tiles = (hidden + rows - 1) / rows * ((live + columns - 1) / columns);
-        const int splits = splits_of(groups, tiles, steps);
         const int64_t stride = live * ld;
         const float *p = part + c * ld + h;
         int s = 0;

@@ -357,14 +357,23 @@ template <int OPEN = 0> __device__ __forceinline__ void wait_and_meet()
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(OPEN) : "memory");
 }
 
-// Into how many parts GX cuts its k: what fills `groups` workgroups with the
-// tokens that count, parts of at least 8 steps.
+// Into how many parts GX cuts its k, up to `groups` workgroups: where the CU with
+// the most parts is done first.  In steps of k: a part has its share of them and
+// about 6 for beginning and end, and every part costs its sums written and read
+// again, 8 bytes for each element of gX (a step of the 256 x 256 tile takes as
+// long as 650000 of them).  All 64 lanes of a wave take part, one possibility
+// each; the answer depends on the arguments alone.
 constexpr int kMaxSplits = 64;
-__device__ __forceinline__ int splits_of(int groups, int tiles, int steps)
+__device__ __forceinline__ int splits_of(int groups, int tiles, int steps, int live, int hidden)
 {
-    int n = tiles > 0 ? groups / tiles : 1;
-    n = n < steps / 8 ? n : steps / 8;
-    return n < 1 ? 1 : (n > kMaxSplits ? kMaxSplits : n);
+    const int lane = threadIdx.x & 63, n = lane + 1;
+    float cost = INFINITY;
+    if (n == 1 || (tiles * n <= groups && n * 4 <= steps))
+        cost = (float)((tiles * n + 255) / 256) * ((float)((steps + n - 1) / n) + 6.0f) +
+               (float)n * ((float)live * (float)hidden / 650000.0f);
+    float least = cost;
+    for (int d = 32; d; d >>= 1) least = fminf(least, __shfl_xor(least, d));
+    return __builtin_ctzll(__builtin_amdgcn_ballot_w64(cost == least)) + 1;
 }
 
 // Which tile of D workgroup `id` computes.  Workgroups go round the 8 XCDs;
@@ -507,7 +516,7 @@ __device__ void Product<T, MODE, BM, BN, WM, WN, BUFFERS, ANY>::run(const Produc
     const int tilesM = (g.M + BM - 1) / BM, tilesN = (boundN + BN - 1) / BN, tiles = tilesM * tilesN;
     int s0 = 0, s1 = (K + kStep<T> - 1) / kStep<T>, split = 0, id = blockIdx.x;
     if constexpr (MODE == GX) {
-        const int splits = splits_of(g.groups, tiles, g.steps), steps = s1;
+        const int splits = splits_of(g.groups, tiles, g.steps, boundN, g.M), steps = s1;
         if (id >= tiles * splits) return;
         split = id / tiles;
         id -= split * tiles;
