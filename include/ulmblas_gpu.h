@@ -506,7 +506,8 @@ int ulmblas_gpu_dlaswp(int n, double *dA, int ldA, int k1, int k2,
  * and results in fp32.  The logits are not kept.  `work`: device memory of
  * ulmblas_gpu_?xent_worksize(hidden, tokens, vocab) bytes, 16-byte aligned, any
  * contents, for one call at a time.  hidden at most 2^20, tokens and vocab at
- * most 2^28 (worksize 0, BAD_ARGUMENT beyond that); tokens == 0 does nothing.
+ * most 2^28 (worksize 0, BAD_ARGUMENT beyond that), ldW below 2^21; tokens == 0
+ * does nothing.
  * Everything is enqueued on `stream`, on the current device; nothing is
  * allocated or synchronised.  The same call gives the same bits. */
 long ulmblas_gpu_sxent_worksize(int hidden, int tokens, int vocab);

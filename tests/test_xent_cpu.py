@@ -51,13 +51,18 @@ def grad(p, hidden=8, tokens=4, vocab=10, ldW=8, ldX=8, ldGW=8, ldGX=8, W=P, X=P
 @pytest.mark.parametrize("p", ["s", "b"])
 def test_refusals_of_the_cross_entropy(p):
     for kw in (dict(hidden=0, ldW=8), dict(hidden=-1), dict(hidden=(1 << 20) + 1, ldW=1 << 21, ldX=1 << 21), dict(tokens=-1),
-               dict(tokens=(1 << 28) + 1), dict(vocab=0), dict(vocab=(1 << 28) + 1), dict(ldW=7), dict(ldX=7), dict(W=None),
-               dict(X=None), dict(label=None), dict(loss=None), dict(lse=None), dict(work=None), dict(work=C.c_void_p(4104))):
+               dict(tokens=(1 << 28) + 1), dict(vocab=0), dict(vocab=(1 << 28) + 1), dict(ldW=7), dict(ldX=7), dict(ldW=1 << 21),
+               dict(W=None), dict(X=None), dict(label=None), dict(loss=None), dict(lse=None), dict(work=None), dict(work=C.c_void_p(4104))):
         assert xent(p, **kw) == BAD, kw
         assert lib.load().ulmblas_gpu_last_error() != b""
     for kw in (dict(hidden=0), dict(tokens=-1), dict(vocab=0), dict(ldW=7), dict(ldX=7), dict(ldGW=7), dict(ldGX=7),
-               dict(W=None), dict(X=None), dict(label=None), dict(lse=None), dict(gloss=None), dict(work=None),
+               dict(ldW=1 << 21), dict(W=None), dict(X=None), dict(label=None), dict(lse=None), dict(gloss=None), dict(work=None),
                dict(work=C.c_void_p(4104))):
+        assert grad(p, **kw) == BAD, kw
+    odd = C.c_void_p(4097)
+    for kw in (dict(W=odd), dict(X=odd), dict(label=odd), dict(loss=odd), dict(lse=odd)):
+        assert xent(p, **kw) == BAD, kw
+    for kw in (dict(W=odd), dict(X=odd), dict(label=odd), dict(lse=odd), dict(gloss=odd), dict(gW=odd), dict(gX=odd)):
         assert grad(p, **kw) == BAD, kw
     # nothing to do: no device is needed
     assert xent(p, tokens=0, W=None, X=None, label=None, loss=None, lse=None, work=None) == 0

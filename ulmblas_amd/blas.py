@@ -467,17 +467,19 @@ class _On:
 
     def __init__(self, device, stream):
         import torch
-        self._guard, self._given, self._device = torch.cuda.device(device), stream, device
+        self._given, self._device = stream, device
+        self._guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
     def __enter__(self):
         import torch
-        self._guard.__enter__()
-        raw = torch.cuda.current_stream(self._device).cuda_stream if self._given is None else self._given
-        self.stream = C.c_void_p(raw)
+        if self._guard is not None:
+            self._guard.__enter__()
+        self.stream = torch.cuda.current_stream().cuda_stream if self._given is None else self._given
         return self
 
     def __exit__(self, *exc):
-        return self._guard.__exit__(*exc)
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
 
     def empty(self, n, dtype):
         """A new tensor whose memory is not handed out again before the work on the stream is done."""

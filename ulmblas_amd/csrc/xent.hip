@@ -247,7 +247,7 @@ gx_kernel(int hidden, const int *__restrict__ place, const int *__restrict__ cou
     vfloat4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     if (c >= 0) {
         if (sizeof(T) == 2) {
-            const float d = delta[rank[c]];
+            const float d = delta[rank ? rank[c] : c];
             const T *w = W + label[c] * ldw + h;
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = e < n ? d * to_float(w[e]) : 0.0f;
@@ -274,7 +274,7 @@ gx_kernel(int hidden, const int *__restrict__ place, const int *__restrict__ cou
 // sizes
 // ---------------------------------------------------------------------------
 
-constexpr int kMaxHidden = 1 << 20, kMaxRows = 1 << 28;
+constexpr int kMaxHidden = 1 << 20, kMaxRows = 1 << 28, kMaxLd = (1 << 21) - 1;
 
 // testing: at most this many vocabulary rows in a piece (0: by size)
 std::atomic<int> g_piece_rows{0};
@@ -305,7 +305,7 @@ int launch_tile(const ProductArgs &g, hipStream_t stream)
         if (dev < 32) ready.fetch_or(1u << dev);
     }
     const int64_t tiles = (int64_t)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN);
-    if (tiles > 0x7fffffff) {
+    if (tiles > 1 << 30) {
         g_last_error = "too many tiles for one launch";
         return ULMBLAS_GPU_BAD_ARGUMENT;
     }
@@ -333,33 +333,43 @@ int launch_tile(const ProductArgs &g, hipStream_t stream)
 //   128 x 64      184    / 605          181    / 596       1.5
 //   128 x 32             / 666                 / 650       1.5
 //
-// The tile for 32 columns is also the one that takes W on any element, so bf16
-// keeps to it there; wider bf16 products would write P past its rows with it.
-// GX may cut k, so that any tile fills the GPU: it counts whole rounds.
+// (bf16 tiles other than the largest lose more with a longer k: 512 tokens, hidden 4096: 150 us against 120.)
+// How many of the tokens count is not known here: all of them decide for three
+// parts, three quarters and half of them for one part each.  The tile for 32
+// columns is bf16's up to 32 tokens (wider products would write P past its rows
+// with it); where W lies off words the logits take it with half its rows (through
+// registers: twice the workgroups keep as many bytes on the way; one token
+// against 1410 x 6230: 92 -> 73 us).  GX may cut k, so that any tile fills the
+// GPU: it counts fractions of rounds.
 struct Tile {
     int rows, columns;
 };
-constexpr Tile kTiles[] = {{256, 256}, {128, 128}, {128, 64}, {128, 32}};
+constexpr Tile kTiles[] = {{256, 256}, {128, 128}, {128, 64}, {128, 32}}, kAnyTile = {64, 32};
 constexpr int kNarrow = 32;
 constexpr int kGroups = 512;            // workgroups GX is spread over: two rounds, so that some tokens may be missing
 
-template <typename T, Mode MODE> Tile choose(int M, int N, int K)
+template <typename T, Mode MODE> Tile choose(int M, int N, int K, bool words = true)
 {
     constexpr bool half = sizeof(T) == 2;
-    if (half && MODE != GW && N <= kNarrow) return kTiles[3];
+    if (half && MODE != GW && N <= kNarrow) return words || MODE == GX ? kTiles[3] : kAnyTile;
     constexpr double rate = half ? 2.44e6 : 0.238e6;            // products and sums a CU and microsecond
-    constexpr double efficiency[4] = {1.0, half ? 0.83 : 0.95, half ? 0.69 : 0.93, 0.84};
+    constexpr double efficiency[4] = {1.0, half ? 0.75 : 0.95, half ? 0.65 : 0.93, 0.84};
     int best = 0;
     double least = 0.0;
     for (int t = 0; t < 4; ++t) {
         if ((MODE == GW && t > 1) || (half && t == 3)) continue;
-        const double tiles = (double)((M + kTiles[t].rows - 1) / kTiles[t].rows) *
-                             ((N + kTiles[t].columns - 1) / kTiles[t].columns);
-        const double rounds = MODE == GX ? std::max(1.0, tiles / 256) : std::ceil(tiles / 256);
-        double k = K, overhead = t == 0 ? 8.5 : 1.5;
-        if (MODE == GX) k = k * std::min(1.0, std::max(tiles / 256, 8.0 * kStep<T> / std::max(K, 1)));
-        if (MODE == GW) overhead = t == 0 ? 12.0 : K <= kStep<T> ? 2.2 : 3.2;
-        const double time = rounds * (kTiles[t].rows * kTiles[t].columns * k / (rate * efficiency[t]) + overhead);
+        double time = 0.0;
+        for (int quarters = 2; quarters <= 4; ++quarters) {
+            const int n = MODE == GW ? N : std::max(1, (int)((int64_t)N * quarters / 4));
+            const int kk = MODE == GW ? std::max(1, (int)((int64_t)K * quarters / 4)) : K;
+            const double tiles = (double)((M + kTiles[t].rows - 1) / kTiles[t].rows) *
+                                 ((n + kTiles[t].columns - 1) / kTiles[t].columns);
+            const double rounds = MODE == GX ? std::max(1.0, tiles / 256) : std::ceil(tiles / 256);
+            double k = kk, overhead = t == 0 ? 8.5 : 1.5;
+            if (MODE == GX) k = k * std::min(1.0, std::max(tiles / 256, 8.0 * kStep<T> / kk));
+            if (MODE == GW) overhead = t == 0 ? 12.0 : K <= kStep<T> ? 2.2 : 3.2;
+            time += (quarters == 4 ? 3 : 1) * rounds * (kTiles[t].rows * kTiles[t].columns * k / (rate * efficiency[t]) + overhead);
+        }
         if (t == 0 || time < least) {
             best = t;
             least = time;
@@ -377,7 +387,7 @@ template <typename T, Mode MODE> int launch_product(const ProductArgs &g, Tile t
     } else {
         if (tile.columns == 32) {
             if constexpr (sizeof(T) == 2)
-                if (!words) return launch_tile<T, MODE, 128, 32, 4, 1, 2, true>(g, stream);
+                if (!words) return launch_tile<T, MODE, MODE == GX ? 128 : 64, 32, 4, 1, 2, true>(g, stream);
             return launch_tile<T, MODE, 128, 32, 4, 1, 4>(g, stream);
         }
         if (tile.columns == 64) return launch_tile<T, MODE, 128, 64, 2, 2, 3>(g, stream);
@@ -391,23 +401,24 @@ template <typename T, Mode MODE> int launch_product(const ProductArgs &g, Tile t
 struct Layout {
     int64_t tokens_p, hidden_p;         // rounded up: rows of compact copies, elements of their rows
     int piece;                          // vocabulary rows at a time (gradient: of P; packing: of W)
-    Tile gx;                            // tile of GX
     int64_t rows, label, place, lse, both, gloss, delta, target, bucket, member, rank, count, x, w, stats, p, part, bytes;
 };
 
-constexpr int64_t kPieceBytes = (int64_t)1 << 30;       // of P or of a packed copy of W, at the most
+// of P and of a packed copy of W in the gradient, and of a packed copy of W in the forward call, at the most
+constexpr int64_t kPieceBytes = (int64_t)1 << 30, kPackBytes = (int64_t)1 << 27;
 
 template <typename T> Layout layout(int hidden, int tokens, int vocab, bool grad)
 {
     Layout l{};
     l.tokens_p = round_up(std::max(tokens, 1), 256);
     l.hidden_p = round_up(hidden, kStep<T>);
-    const int64_t row = std::max(grad ? l.tokens_p : 0, l.hidden_p) * (int64_t)sizeof(T);
-    int64_t piece = std::max<int64_t>(kPieceBytes / row / 256 * 256, 256);
-    piece = std::min<int64_t>(piece, 1 << 19);
-    if (g_piece_rows.load() > 0) piece = std::min<int64_t>(piece, round_up(g_piece_rows.load(), 256));
-    l.piece = (int)std::min<int64_t>(piece, round_up(vocab, 256));
-    l.gx = choose<T, GX>(hidden, std::max(tokens, 1), l.piece);
+    // bf16 may have to pack its piece of W; a piece is at most 2^19 rows, and all are about as long
+    const bool packs = sizeof(T) == 2 && tokens > kNarrow;
+    const int64_t row = std::max(grad ? l.tokens_p : 1, packs ? l.hidden_p : 1) * (int64_t)sizeof(T);
+    int64_t most = std::min<int64_t>(std::max<int64_t>((grad ? kPieceBytes : kPackBytes) / row / 256 * 256, 256), 1 << 19);
+    if (g_piece_rows.load() > 0) most = std::min<int64_t>(most, round_up(g_piece_rows.load(), 256));
+    const int64_t pieces = (vocab + most - 1) / most;
+    l.piece = (int)round_up((vocab + pieces - 1) / pieces, 256);
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t here = at;
@@ -429,24 +440,25 @@ template <typename T> Layout layout(int hidden, int tokens, int vocab, bool grad
         l.bucket = take(4 * (round_up(vocab, 128) / 128 + 1));
     }
     l.x = take(l.tokens_p * l.hidden_p * (int64_t)sizeof(T));
-    l.w = take((int64_t)l.piece * l.hidden_p * (int64_t)sizeof(T));
+    l.w = take(packs ? (int64_t)l.piece * l.hidden_p * (int64_t)sizeof(T) : 0);
     if (!grad) {
-        l.stats = take((round_up(vocab, 256) / 128) * l.tokens_p * 8);
+        l.stats = take((round_up(vocab, 256) / kAnyTile.rows) * l.tokens_p * 8);
     } else {
         l.p = take(l.tokens_p * l.piece * (int64_t)sizeof(T));
         // as many splits as fill kGroups workgroups with tiles, or one
-        l.part = take(std::max((int64_t)kGroups * l.gx.rows * l.gx.columns, l.tokens_p * l.hidden_p) * 4);
+        const Tile gx = choose<T, GX>(hidden, std::max(tokens, 1), l.piece);
+        l.part = take(std::max((int64_t)kGroups * gx.rows * gx.columns, l.tokens_p * l.hidden_p) * 4);
     }
     l.bytes = at;
     return l;
 }
 
 // Whether W's rows start on 4 bytes, as the copies straight into LDS need them, and whether the product kernel can read
-// W where it lies: then, or with the tile for few tokens; a tile's rows are within 31 bits of each other.
+// W where it lies: then, or with the tile for few tokens.
 template <typename T> bool on_words(const T *W, int ldW) { return ((uintptr_t)W & 3) == 0 && ldW * sizeof(T) % 4 == 0; }
 template <typename T> bool in_place(const T *W, int ldW, int tokens)
 {
-    return (on_words(W, ldW) || tokens <= kNarrow) && (int64_t)ldW * (int64_t)sizeof(T) < (1 << 23);
+    return on_words(W, ldW) || tokens <= kNarrow;
 }
 
 template <typename T>
@@ -481,6 +493,8 @@ int bad(const char *text)
     return ULMBLAS_GPU_BAD_ARGUMENT;
 }
 
+template <typename T> bool off(const void *p) { return (uintptr_t)p % sizeof(T) != 0; }
+
 template <typename T> T *part_of(void *work, int64_t at) { return reinterpret_cast<T *>(static_cast<char *>(work) + at); }
 
 template <typename T>
@@ -489,8 +503,11 @@ int xent_device(int hidden, int tokens, int vocab, float alpha, const T *W, int 
 {
     if (!sizes_ok(hidden, tokens, vocab)) return bad("invalid size");
     if (ldW < hidden || ldX < hidden) return bad("leading dimension smaller than hidden");
+    if (ldW > kMaxLd) return bad("leading dimension of W beyond 2^21");
     if (tokens == 0) return ULMBLAS_GPU_OK;
     if (!W || !X || !label || !loss || !lse || !work) return bad("null operand or workspace");
+    if (off<T>(W) || off<T>(X) || off<int>(label) || off<float>(loss) || off<float>(lse))
+        return bad("operand off its type's alignment");
     if ((uintptr_t)work & 15) return bad("workspace not on 16 bytes");
     const Layout l = layout<T>(hidden, tokens, vocab, false);
     TokenArgs t{};
@@ -537,7 +554,7 @@ int xent_device(int hidden, int tokens, int vocab, float alpha, const T *W, int 
             g.widthA = (int)l.hidden_p;
         }
         g.stats = part_of<float2>(work, l.stats) + (int64_t)tiles * l.tokens_p;
-        const Tile tile = choose<T, STATS>(g.M, g.N, g.K);
+        const Tile tile = choose<T, STATS>(g.M, g.N, g.K, words);
         if ((rc = launch_product<T, STATS>(g, tile, words, stream))) return rc;
         tiles += (g.M + tile.rows - 1) / tile.rows;
     }
@@ -560,9 +577,13 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
     if (!sizes_ok(hidden, tokens, vocab)) return bad("invalid size");
     if (ldW < hidden || ldX < hidden || (gW && ldGW < hidden) || (gX && ldGX < hidden))
         return bad("leading dimension smaller than hidden");
+    if (ldW > kMaxLd) return bad("leading dimension of W beyond 2^21");
     if (!gW && !gX) return ULMBLAS_GPU_OK;
     if (tokens > 0 && (!W || !X || !label || !lse || !gloss)) return bad("null operand");
     if (!work) return bad("null workspace");
+    if (off<T>(W) || off<T>(X) || off<T>(gW) || off<T>(gX) || off<int>(label) || off<float>(lse) || off<float>(gloss) ||
+        off<float>(glse))
+        return bad("operand off its type's alignment");
     if ((uintptr_t)work & 15) return bad("workspace not on 16 bytes");
     const Layout l = layout<T>(hidden, tokens, vocab, true);
     TokenArgs t{};
@@ -586,8 +607,8 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
     if (rc) return rc;
     float *delta = part_of<float>(work, l.delta);
     int2 *member = part_of<int2>(work, l.member);
-    int *rank = part_of<int>(work, l.rank), *bucket = part_of<int>(work, l.bucket);
-    if (sizeof(T) == 2) {
+    int *rank = tokens > kUnsorted ? part_of<int>(work, l.rank) : nullptr, *bucket = part_of<int>(work, l.bucket);
+    if (sizeof(T) == 2 && tokens > kUnsorted) {
         hipLaunchKernelGGL(bucket_kernel, dim3((unsigned)(round_up(vocab, 128) / 128 + 1)), dim3(256), 0, stream, t.count,
                            t.label_c, member, rank, bucket);
         HIP_TRY(hipGetLastError());
@@ -596,6 +617,7 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
     const int64_t row_x = l.hidden_p * (int64_t)sizeof(T), row_p = (int64_t)l.piece / kStep<T> * kBlockBytes;
     const int blocks_p = (int)(l.tokens_p / kBlockTokens * (l.piece / kStep<T>));
     const bool direct = in_place(W, ldW, tokens), words = !direct || on_words(W, ldW);
+    const Tile gx_tile = choose<T, GX>(hidden, std::max(tokens, 1), l.piece);
     for (int v0 = 0; v0 < vocab; v0 += l.piece) {
         const int vn = std::min(l.piece, vocab - v0);
         const T *Wv = W ? W + (int64_t)v0 * ldW : nullptr;
@@ -630,7 +652,7 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
             g.ldP = row_p;
             g.rank = rank;
             g.delta = delta;
-            if ((rc = launch_product<T, PROB>(g, choose<T, PROB>(g.M, g.N, g.K), words, stream))) return rc;
+            if ((rc = launch_product<T, PROB>(g, choose<T, PROB>(g.M, g.N, g.K, words), words, stream))) return rc;
         }
         if (gX && tokens > 0) {
             g.A = Wv;
@@ -647,7 +669,7 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
             g.groups = kGroups;
             g.steps = (l.piece + kStep<T> - 1) / kStep<T>;
             g.add = v0 > 0;
-            if ((rc = launch_product<T, GX>(g, l.gx, words, stream))) return rc;
+            if ((rc = launch_product<T, GX>(g, gx_tile, words, stream))) return rc;
         }
         if (gW) {
             g.A = Xc;
@@ -660,6 +682,8 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
             g.N = vn;
             g.K = tokens;
             g.first = v0;
+            g.label = t.label_c;
+            g.rank = rank;
             g.delta = delta;
             g.bucket = bucket;
             g.member = member;
@@ -671,7 +695,7 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
     }
     if (gX && tokens > 0) {
         hipLaunchKernelGGL(gx_kernel<T>, dim3((unsigned)tokens, (unsigned)((hidden + 1023) / 1024)), dim3(256), 0, stream, hidden, t.place,
-                           t.count, l.gx.rows, l.gx.columns, kGroups, (l.piece + kStep<T> - 1) / kStep<T>,
+                           t.count, gx_tile.rows, gx_tile.columns, kGroups, (l.piece + kStep<T> - 1) / kStep<T>,
                            part_of<float>(work, l.part), l.hidden_p, delta, rank,
                            t.label_c, W, (int64_t)ldW, gX,
                            (int64_t)ldGX);

@@ -101,7 +101,7 @@ struct ProductArgs {
     const float *lse, *both, *gloss;    // per token; both = gloss + glse, each times alpha
     void *P;
     int64_t ldP;                // bytes from one row of blocks to the next
-    const int *rank;            // per token: its place in `member`
+    const int *rank;            // per token: its place in `member` (null: the tokens are too few to be sorted)
     float *delta;               // per place there: what rounding took from P at the label (PROB writes, GW reads)
     // GX: partial sums of the splits, each [token][ldD], one after the other as long as `count` makes them
     float *part;
@@ -368,7 +368,7 @@ __device__ __forceinline__ int splits_of(int groups, int tiles, int steps, int l
 {
     const int lane = threadIdx.x & 63, n = lane + 1;
     float cost = INFINITY;
-    if (n == 1 || (tiles * n <= groups && n * 4 <= steps))
+    if (n == 1 || (tiles <= groups / n && n * 4 <= steps))
         cost = (float)((tiles * n + 255) / 256) * ((float)((steps + n - 1) / n) + 6.0f) +
                (float)n * ((float)live * (float)hidden / 650000.0f);
     float least = cost;
@@ -445,23 +445,25 @@ template <typename T> __device__ __forceinline__ int64_t p_byte(int n, int m, in
 // The tile of gW^T starts from what rounding took from P at the labels: for
 // every token whose label is one of the tile's columns, delta times its x.  The
 // tokens are found through the groups of 128 vocabulary rows they are sorted by,
-// 64 of them at a time, and those of this wave's columns are taken in pairs, so
-// that their rows of x are on the way together; all of it runs while the first
-// step is fetched.
+// 64 of them at a time (up to 64 tokens are not sorted: every tile looks at all),
+// and those of this wave's columns are taken in pairs, so that their rows of x
+// are on the way together; all of it runs while the first step is fetched.
+constexpr int kUnsorted = 64;
 template <typename T, int BM, int BN, int WM, int WN>
 __device__ __forceinline__ void add_label_remainders(const ProductArgs &g, int m0, int n0, int wm, int wn, int lane,
-                                                     vfloat4 (&acc)[BM / WM / 16][BN / WN / 16])
+                                                     int live, vfloat4 (&acc)[BM / WM / 16][BN / WN / 16])
 {
     constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
     const int v0 = g.first + n0, v1 = v0 + BN < g.first + g.N ? v0 + BN : g.first + g.N;
-    const int from = __builtin_amdgcn_readfirstlane(g.bucket[v0 / 128]);
-    const int to = __builtin_amdgcn_readfirstlane(g.bucket[(v1 + 127) / 128]);
+    const int from = g.rank ? __builtin_amdgcn_readfirstlane(g.bucket[v0 / 128]) : 0;
+    const int to = g.rank ? __builtin_amdgcn_readfirstlane(g.bucket[(v1 + 127) / 128]) : live;
     for (int e0 = from; e0 < to; e0 += 64) {
         const int e = e0 + lane < to ? e0 + lane : to - 1;
-        const int2 member = g.member[e];
+        const int2 member = g.rank ? g.member[e] : make_int2(e, g.label[e]);
         const float delta = g.delta[e];
         const int column = member.y - v0;
-        unsigned long long mine = __builtin_amdgcn_ballot_w64(e0 + lane < to && column / (TN * 16) == wn);
+        unsigned long long mine =
+            __builtin_amdgcn_ballot_w64(e0 + lane < to && column >= 0 && column < v1 - v0 && column / (TN * 16) == wn);
         while (mine) {
             int n[2];
             float d[2];
@@ -624,7 +626,7 @@ __device__ void Product<T, MODE, BM, BN, WM, WN, BUFFERS, ANY>::run(const Produc
 #pragma unroll
         for (int c = 0; c < kCalls; ++c) call(c);
         if constexpr (MODE == GW && sizeof(T) == 2)
-            add_label_remainders<T, BM, BN, WM, WN>(g, m0, n0, wm, wn, lane, acc);
+            add_label_remainders<T, BM, BN, WM, WN>(g, m0, n0, wm, wn, lane, live, acc);
 #pragma unroll
         for (int x = 1; x + 1 < BUFFERS; ++x) {
             aim(s0 + x, x * kStage);
@@ -780,7 +782,7 @@ __device__ void Product<T, MODE, BM, BN, WM, WN, BUFFERS, ANY>::run(const Produc
                         if (mw + i * 16 + r == want) {
                             const float p = acc[i][j][r] - gloss;
                             acc[i][j][r] = p;
-                            if constexpr (sizeof(T) == 2) g.delta[g.rank[n]] = p - to_float(from_float<T>(p));
+                            if constexpr (sizeof(T) == 2) g.delta[g.rank ? g.rank[n] : n] = p - to_float(from_float<T>(p));
                         }
             }
             if (tail || n0 + BN > boundN) {
