@@ -107,7 +107,7 @@ class Problem:
 
 SIZES = [  # hidden, tokens, vocab
     (1, 1, 1), (8, 1, 2), (64, 1, 1000), (65, 7, 257), (96, 16, 300), (72, 17, 4097), (200, 33, 640), (1000, 130, 777),
-    (512, 300, 5000), (40, 257, 511), (4097, 3, 130),
+    (512, 300, 5000), (40, 257, 511), (4097, 3, 130), (300, 8, 9000), (72, 9, 2049), (8200, 2, 300),
 ]
 
 
@@ -117,6 +117,18 @@ def test_sizes(prec, hidden, tokens, vocab):
     p = Problem(prec, hidden, tokens, vocab, seed=hidden + tokens)
     p.check_forward()
     p.check_backward()
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+@pytest.mark.parametrize("hidden", [7, 511, 513, 4096, 4097, 8191])
+@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 6, 8])
+def test_few_tokens(prec, hidden, tokens):
+    """One pass over W, for every number of tokens, one and two stretches of elements a thread."""
+    p = Problem(prec, hidden, tokens, 67, pad=hidden % 3, off=hidden % 5, seed=hidden + tokens, masked=0.3)
+    p.check_forward()
+    p.check_backward(beta=0.5, pad_out=1)
+    p.check_backward(glse=False, want=("X",))
+    p.check_backward(want=("W",))
 
 
 @pytest.mark.parametrize("prec", ["s", "b"])
@@ -133,7 +145,7 @@ def test_large_tiles(prec):
 @pytest.mark.parametrize("prec", ["s", "b"])
 @pytest.mark.parametrize("pad,off", [(1, 0), (0, 1), (8, 8), (3, 5)])
 def test_strides_and_alignment(prec, pad, off):
-    for hidden, tokens, vocab in ((128, 5, 515), (136, 140, 700)):
+    for hidden, tokens, vocab in ((128, 5, 515), (129, 12, 515), (136, 140, 700)):
         p = Problem(prec, hidden, tokens, vocab, pad=pad, off=off, alpha=0.7, masked=0.3, seed=pad * 10 + off)
         p.check_forward()
         p.check_backward(pad_out=pad, off_out=off, beta=0.5)
@@ -197,7 +209,7 @@ def test_ignore_may_be_a_row_of_the_classifier(prec):
 
 
 @pytest.mark.parametrize("prec", ["s", "b"])
-@pytest.mark.parametrize("tokens", [3, 140])
+@pytest.mark.parametrize("tokens", [3, 20, 140])
 def test_pieces_of_the_vocabulary(prec, tokens):
     p = Problem(prec, 200, tokens, 1500, seed=11, masked=0.2)
     q = Problem(prec, 200, tokens, 1500, pad=1, seed=12, masked=0.2)        # packed
