@@ -66,6 +66,14 @@ int gemm_tri_device(int tri, bool ta, bool tb, int n, int k, T alpha, const T *d
 void lu_set_spin_limit(long polls);
 // Testing: every LU panel takes the path of many small launches that wait for nobody.
 void lu_set_simple_panels(bool on);
+// The cross entropy's gradient for up to 8 tokens in one pass over W (xent_few.hip; float and bf16 bits): whether it takes
+// a problem, the bytes it needs, and the call (arguments checked by the caller).
+bool xent_takes_few(int hidden, int tokens);
+long xent_few_worksize(int hidden, int tokens, int vocab);
+template <typename T>
+int xent_few_grad(int hidden, int tokens, int vocab, float alpha, const T *W, int ldW, const T *X, int ldX, const int *label,
+                  int ignore, const float *lse, const float *gloss, const float *glse, float beta, T *gW, int ldGW, T *gX,
+                  int ldGX, float *work, hipStream_t stream);
 void xent_set_piece_rows(int rows);   // vocabulary rows the cross entropy's gradient takes at a time (testing)
 int trsm_set_parts(int parts);   // blocks of unknowns per launch of the triangular solve (testing)
 
