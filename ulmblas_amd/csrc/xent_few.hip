@@ -14,11 +14,12 @@
 //
 // P stays in fp32.  The next rows are on their way while these are worked on.
 // Measured (vocabulary 32768, hidden 4096): bf16 1 - 2 tokens 108 us and 4 tokens
-// 118 us, which the bytes of W and gW bound (4.5 - 5.0 TB/s), 8 tokens 165 us, bound by
+// 118 us, which the bytes of W and gW bound (4.5 - 5.0 TB/s), 8 tokens 165 - 175 us, bound by
 // the 24 multiplications and additions an element of W and their operands' conversion;
-// fp32 205 - 233 us.  The three products as such take 230 and 410 us.  5 x 1001 x 30001
-// bf16: 46 us (70 us by the products).  A kernel for each count of tokens: with values
-// for the next power of two computed too, 5 tokens took 55 us there.
+// fp32 205 - 233 us.  The three products as such take 230 and 415 us.  5 x 1001 x 30001
+// bf16: 43 us (70 us by the products), 36 of them in this pass: rows off their alignment,
+// and W read at half of memory's rate.  A kernel for each count of tokens: with values
+// for the next power of two computed too, that pass took 46 us.
 // The exchange between lanes goes through swaps and DPP: through LDS it was the
 // longest part of the work on a set of rows (2 tokens, hidden 1024: 83 -> 34 us).
 
@@ -191,10 +192,8 @@ __global__ void __launch_bounds__(512, 2) few_kernel(FewArgs g)
     const int stride = (int)gridDim.x * ROWS;
     int parity = 0;
     fetch(w, blockIdx.x * ROWS);
-    bool more = (int)blockIdx.x * ROWS < g.vocab;
-    for (int v0 = blockIdx.x * ROWS; more; v0 += more ? stride : 0) {
-        more = g.vocab - v0 > stride;               // so that no sum passes 32 bits
-        if (more) fetch(next, v0 + stride);
+    for (int v0 = blockIdx.x * ROWS; v0 < g.vocab; v0 += stride) {
+        if (v0 + stride < g.vocab) fetch(next, v0 + stride);
         float z[N];
 #pragma unroll
         for (int r = 0; r < ROWS; ++r)
@@ -277,13 +276,16 @@ __global__ void __launch_bounds__(512, 2) few_kernel(FewArgs g)
 }
 
 // gX of the pass above: 64 elements of one token a workgroup, 16 threads with
-// four elements each and 16 of those side by side along the parts.
+// four elements each and `slices` (at most 64) of those side by side along the
+// parts: one for 16 parts, so that reads in flight hide their latency (1024 parts of
+// 5 x 1001: 16 slices 10 us, 64 slices 6.8 us).
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 few_gx_kernel(int hidden, int tokens, int vocab, int ignore, const int *__restrict__ label, const float *__restrict__ part,
               int parts, T *gx, int64_t ldgx)
 {
-    __shared__ float sums[16][64];
+    __shared__ float sums[64][64];
+    const int slices = blockDim.x >> 4;
     const int t = blockIdx.x, h = blockIdx.y * 64 + (threadIdx.x & 15) * 4, slice = threadIdx.x >> 4, y = label[t];
     const bool counts = y != ignore && y >= 0 && y < vocab;
     const int n = hidden - h;
@@ -302,22 +304,22 @@ few_gx_kernel(int hidden, int tokens, int vocab, int ignore, const int *__restri
     };
     if (counts) {
         int k = slice;
-        for (; k + 7 * 16 < parts; k += 8 * 16) {
+        for (; k + 7 * slices < parts; k += 8 * slices) {
             vfloat4 a[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) a[u] = one(k + u * 16);
+            for (int u = 0; u < 8; ++u) a[u] = one(k + u * slices);
 #pragma unroll
             for (int u = 0; u < 8; ++u) v += a[u];
         }
-        for (; k < parts; k += 16) v += one(k);
+        for (; k < parts; k += slices) v += one(k);
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) sums[slice][(threadIdx.x & 15) * 4 + e] = v[e];
     __syncthreads();
     if (threadIdx.x < 64 && blockIdx.y * 64 + threadIdx.x < (unsigned)hidden) {
         float s = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) s += sums[k][threadIdx.x];
+#pragma unroll 16
+        for (int k = 0; k < slices; ++k) s += sums[k][threadIdx.x];
         gx[t * ldgx + blockIdx.y * 64 + threadIdx.x] = from_float<T>(s);
     }
 }
@@ -371,7 +373,8 @@ int xent_few_grad(int hidden, int tokens, int vocab, float alpha, const T *W, in
     case 8: rc = launch_few<T, 8>(f, parts, stream); break;
     }
     if (rc || !gX) return rc;
-    hipLaunchKernelGGL(few_gx_kernel<T>, dim3((unsigned)tokens, (unsigned)((hidden + 63) / 64)), dim3(256), 0, stream, hidden,
+    const int slices = std::min(std::max(parts / 16, 16), 64);
+    hipLaunchKernelGGL(few_gx_kernel<T>, dim3((unsigned)tokens, (unsigned)((hidden + 63) / 64)), dim3(16 * slices), 0, stream, hidden,
                        tokens, vocab, ignore, label, work, parts, gX, (int64_t)ldGX);
     HIP_TRY(hipGetLastError());
     return ULMBLAS_GPU_OK;
