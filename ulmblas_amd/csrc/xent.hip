@@ -693,6 +693,7 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
             g.out = gW + (int64_t)v0 * ldGW;
             g.ldD = ldGW;
             g.beta = beta;
+            g.past = (int64_t)vocab * hidden * (int64_t)sizeof(T) > kPastCaches;
             if ((rc = launch_product<T, GW>(g, choose<T, GW>(g.M, g.N, g.K), words, stream))) return rc;
         }
     }

@@ -110,6 +110,7 @@ struct ProductArgs {
     // GW
     void *out;
     float beta;
+    bool past;                  // bf16's gW goes past the caches (kPastCaches)
     const int *bucket;          // first place of each group of 128 vocabulary rows
     const int2 *member;         // tokens (compact) in the order of their label's group, and their labels
 };
@@ -417,9 +418,17 @@ template <int BM> __device__ __forceinline__ int staged_at(int row, int col)
     return row * (BM * 2) + (((col >> 3) ^ (row & (kChunks - 1))) << 4) + (col & 7) * 2;
 }
 
+// Beyond this many bytes bf16's gW is stored with the hint that nobody reads it soon: it does not fit the memory's cache
+// of 256 MB, and without it what W, X and P have there stays (512 x 4096 x 32768: 509 -> 503 us; 8192 x 4096 x 131072:
+// 21.9 -> 21.7 ms).  Below, whoever reads gW next finds it there (with the norm and the clipping behind it, 1024 x
+// 2048 x 32768: 520 us, with the hint 528; 1024 x 4096 x 65536: 1900 and 1843 us).  Only whole rows gain: fp32 stores 16
+// bytes a lane across rows (256 x 4096 x 32768: 1660 us, with the hint 1690), and the pass for few tokens
+// half of a thread's 32 bytes at a time (1 x 4096 x 32768: 205 us, with the hint 334).
+constexpr int64_t kPastCaches = (int64_t)1 << 28;
+
 // Writes the staged tile out, whole rows at a time: rows x cols of it.
 template <int BM, int THREADS>
-__device__ __forceinline__ void write_staged(const unsigned char *lds, bf16_t *to, int64_t ld, int rows, int cols)
+__device__ __forceinline__ void write_staged(const unsigned char *lds, bf16_t *to, int64_t ld, int rows, int cols, bool past)
 {
     constexpr int kChunks = BM / 8;
     for (int i = threadIdx.x; i < rows * kChunks; i += THREADS) {
@@ -428,7 +437,14 @@ __device__ __forceinline__ void write_staged(const unsigned char *lds, bf16_t *t
         const unsigned char *v = lds + staged_at<BM>(row, col);
         bf16_t *p = to + row * ld + col;
         if (col + 8 <= cols) {
-            *reinterpret_cast<AnyVector<bf16_t>::V *>(p) = *reinterpret_cast<const vint4 *>(v);
+            auto *wide = reinterpret_cast<AnyVector<bf16_t>::V *>(p);
+            if (past) {
+                asm volatile("; past the caches");          // else the compiler joins the two stores and drops the hint
+                __builtin_nontemporal_store(*reinterpret_cast<const vint4 *>(v), wide);
+                asm volatile("; stored");
+            } else {
+                *wide = *reinterpret_cast<const vint4 *>(v);
+            }
         } else {
             for (int e = 0; e < cols - col; ++e) p[e] = reinterpret_cast<const bf16_t *>(v)[e];
         }
@@ -447,7 +463,10 @@ template <typename T> __device__ __forceinline__ int64_t p_byte(int n, int m, in
 // tokens are found through the groups of 128 vocabulary rows they are sorted by,
 // 64 of them at a time (up to 64 tokens are not sorted: every tile looks at all),
 // and those of this wave's columns are taken in pairs, so that their rows of x
-// are on the way together; all of it runs while the first step is fetched.
+// are on the way together.  It is done before the first step is asked for: loads come
+// back in order, and these would wait for all of it (8192 x 4096 x 131072: 21.7 -> 21.4
+// ms; the part that is left, 20 of the 170 us of 1024 x 2048 x 32768, is one in four
+// of these multiplications meeting a label).
 constexpr int kUnsorted = 64;
 template <typename T, int BM, int BN, int WM, int WN>
 __device__ __forceinline__ void add_label_remainders(const ProductArgs &g, int m0, int n0, int wm, int wn, int lane,
@@ -486,13 +505,16 @@ __device__ __forceinline__ void add_label_remainders(const ProductArgs &g, int m
             }
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
+                float dj[TN];
+#pragma unroll
+                for (int j = 0; j < TN; ++j) dj[j] = n[p] / 16 == j ? d[p] : 0.0f;
 #pragma unroll
                 for (int i = 0; i < TM; ++i) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float f = d[p] * to_float((bf16_t)((unsigned)x[p][i][r >> 1] >> 16 * (r & 1)));
+                        const float f = to_float((bf16_t)((unsigned)x[p][i][r >> 1] >> 16 * (r & 1)));
 #pragma unroll
-                        for (int j = 0; j < TN; ++j) acc[i][j][r] += n[p] / 16 == j ? f : 0.0f;
+                        for (int j = 0; j < TN; ++j) acc[i][j][r] = fmaf(dj[j], f, acc[i][j][r]);
                     }
                     __builtin_amdgcn_sched_barrier(0);      // keeps the unpacked values of one row of tiles at a time
                 }
@@ -622,11 +644,11 @@ __device__ void Product<T, MODE, BM, BN, WM, WN, BUFFERS, ANY>::run(const Produc
         // Steps past the end are asked for too where more than two tiles are open (they bring zeros), so that what
         // is open is the same number of calls in every step.
         constexpr int kOpen = (BUFFERS - 2) * kCalls;
+        if constexpr (MODE == GW && sizeof(T) == 2)
+            add_label_remainders<T, BM, BN, WM, WN>(g, m0, n0, wm, wn, lane, live, acc);
         aim(s0, 0);
 #pragma unroll
         for (int c = 0; c < kCalls; ++c) call(c);
-        if constexpr (MODE == GW && sizeof(T) == 2)
-            add_label_remainders<T, BM, BN, WM, WN>(g, m0, n0, wm, wn, lane, live, acc);
 #pragma unroll
         for (int x = 1; x + 1 < BUFFERS; ++x) {
             aim(s0 + x, x * kStage);
@@ -867,7 +889,7 @@ __device__ void Product<T, MODE, BM, BN, WM, WN, BUFFERS, ANY>::run(const Produc
         if constexpr (sizeof(T) == 2) {
             __syncthreads();
             write_staged<BM, kThreads>(lds_raw, out + (int64_t)n0 * g.ldD + m0, g.ldD, g.N - n0 < BN ? g.N - n0 : BN,
-                                       g.M - m0 < BM ? g.M - m0 : BM);
+                                       g.M - m0 < BM ? g.M - m0 : BM, g.past);
         }
     }
 }
