@@ -529,7 +529,8 @@ int ulmblas_gpu_bxent(int hidden, int tokens, int vocab, float alpha,
  *     gW = alpha * X * P^T + beta * gW      (hidden x vocab)
  * beta == 0 never reads gW.  A null dGW or dGX is not computed.  The logits are
  * computed again, a piece of the vocabulary at a time, and P of that piece is
- * rounded to the operands' type for the two products.  Outputs must not overlap
+ * rounded to the operands' type for the two products (up to 8 tokens it is not:
+ * hidden up to 4096, or 8192 with up to 4 tokens).  Outputs must not overlap
  * inputs, each other or `work` (ulmblas_gpu_?xent_grad_worksize bytes). */
 long ulmblas_gpu_sxent_grad_worksize(int hidden, int tokens, int vocab);
 long ulmblas_gpu_bxent_grad_worksize(int hidden, int tokens, int vocab);
