@@ -505,9 +505,9 @@ int ulmblas_gpu_dlaswp(int n, double *dA, int ldA, int k1, int k2,
  * whatever it holds.  s: fp32 operands; b: bf16 operands (their 16 bits), sums
  * and results in fp32.  The logits are not kept.  `work`: device memory of
  * ulmblas_gpu_?xent_worksize(hidden, tokens, vocab) bytes, 16-byte aligned, any
- * contents, for one call at a time.  hidden at most 2^20, tokens and vocab at
- * most 2^28 (worksize 0, BAD_ARGUMENT beyond that), ldW below 2^21; tokens == 0
- * does nothing.
+ * contents, for one call at a time.  hidden at most 2^20, tokens at most 2^23,
+ * vocab at most 2^28 (worksize 0, BAD_ARGUMENT beyond that), ldW below 2^21;
+ * tokens == 0 does nothing.
  * Everything is enqueued on `stream`, on the current device; nothing is
  * allocated or synchronised.  The same call gives the same bits. */
 long ulmblas_gpu_sxent_worksize(int hidden, int tokens, int vocab);
@@ -557,7 +557,8 @@ int ulmblas_gpu_bxent_grad(int hidden, int tokens, int vocab, float alpha,
  * group).  `work`: device memory of ulmblas_gpu_gnrm2_worksize(count) bytes,
  * 8-byte aligned, any contents, for one call at a time.
  * gclip: dY[i] = dX[i] * min(1, largest / *dNorm), elementwise, dNorm on the
- * device; dY[i] is dX[i] itself or does not overlap any tensor of the group.
+ * device; dY[i] is dX[i] itself or does not overlap any tensor of the group, and
+ * no two dY overlap (so a tensor is in a group that is scaled in place once).
  * A norm that is infinite or no number leaves the values as they are.  Nothing
  * is allocated or synchronised; the same call gives the same bits. */
 long ulmblas_gpu_gnrm2_worksize(int count);

@@ -151,3 +151,23 @@ def test_outputs_of_other_kinds_are_refused():
         blas.gpu_gclip([x], norm, -1.0)
     with pytest.raises(ValueError):
         blas.gpu_gnrm2([x], work=torch.empty(8, dtype=torch.uint8, device="cuda"))
+
+
+def test_overlapping_tensors_are_not_scaled():
+    """A tensor that is in the group twice would be scaled twice, or by what the other one left."""
+    import torch
+    flat, norm = torch.arange(64, device="cuda", dtype=torch.float32), torch.ones(1, device="cuda")
+    a, b, c = flat[:32], flat[31:48], flat[48:]
+    for tensors in ([a, a], [a, c, b], [flat, b[:0], c]):
+        group = blas.TensorGroup(tensors)
+        for _ in range(2):
+            with pytest.raises(ValueError, match="overlaps"):
+                blas.gpu_gclip(group, norm, 0.5)
+    for tensors, out in (([a, c], [c.new_empty(32), a[:16]]), ([a, c], [flat[16:48], c]), ([a[:16], c], [b[:16], b[1:17]])):
+        with pytest.raises(ValueError, match="overlaps"):
+            blas.gpu_gclip(tensors, norm, 0.5, out=out)
+    assert (flat.cpu() == torch.arange(64)).all()
+    # the norm counts a tensor as often as it is named; neighbours are fine, and so are tensors of no length inside others
+    assert abs(float(blas.gpu_gnrm2([c, c])) - float(c.double().norm()) * 2 ** 0.5) < 1e-3
+    blas.gpu_gclip([a, flat[32:48], c, flat[40:40]], norm, 0.5)
+    assert (flat.cpu() == torch.arange(64) * 0.5).all()

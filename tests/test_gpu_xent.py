@@ -352,3 +352,90 @@ def test_two_calls_at_once(prec):
         torch.cuda.synchronize()
         for (l, e), (wl, we) in zip(got, want):
             assert np.array_equal(l.double().cpu().numpy(), wl) and np.array_equal(e.double().cpu().numpy(), we)
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+def test_most_tokens(prec):
+    """As many tokens as a call takes: offsets of P pass 32 bits.  All but 2000 of them have gradient 0, so that these
+    (the first and the last ones among them) are all that a result holds."""
+    import torch
+    H, T, V = 12, 1 << 23, 300
+    dt = {"s": torch.float32, "b": torch.bfloat16}[prec]
+    gen = torch.Generator("cuda").manual_seed(3)
+    X = torch.randn(T, H, generator=gen, device="cuda").to(dt)
+    W = torch.randn(V, H, generator=gen, device="cuda").to(dt)
+    label = torch.randint(0, V, (T,), generator=gen, device="cuda", dtype=torch.int32)
+    label[1000:T // 2:7] = IGNORE
+    loss, lse = blas.gpu_xent(prec, H, T, V, 1.0, W, H, X, H, label)
+    torch.cuda.synchronize()
+    assert torch.isfinite(loss).all() and torch.isfinite(lse).all() and (loss[label == IGNORE] == 0).all()
+    some = torch.cat([torch.arange(500), torch.arange(T // 2 - 500, T // 2 + 500), torch.arange(T - 500, T)])
+    at = some.cuda()
+    w64, x64, y = W.double().cpu().numpy(), X[at].double().cpu().numpy(), label[at].cpu().numpy()
+    wloss, wlse, blse, bloss = xent_ref.forward(w64, x64, y, 1.0, IGNORE, prec)
+    assert (np.abs(lse[at].double().cpu().numpy() - wlse) <= blse).all()
+    assert (np.abs(loss[at].double().cpu().numpy() - wloss) <= bloss).all()
+    gloss = torch.zeros(T, device="cuda")
+    gloss[at] = torch.randn(len(some), generator=gen, device="cuda")
+    gW, gX = torch.full_like(W, float("nan")), torch.full_like(X, float("nan"))
+    blas.gpu_xent_grad(prec, H, T, V, 1.0, W, H, X, H, label, IGNORE, lse, gloss, None, 0.0, gW, H, gX, H)
+    torch.cuda.synchronize()
+    wW, wX, bW, bX = xent_ref.backward(w64, x64, y, 1.0, IGNORE, lse[at].double().cpu().numpy(),
+                                       gloss[at].double().cpu().numpy(), None, prec)
+    assert (np.abs(gW.double().cpu().numpy() - wW) <= bW).all()
+    assert (np.abs(gX[at].double().cpu().numpy() - wX) <= bX).all()
+    gX[at] = 0
+    assert (gX == 0).all()
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+@pytest.mark.parametrize("tokens", [3, 20, 90])
+def test_classifier_past_32_bits(prec, tokens):
+    """W and gW of more than 2^31 elements.  Only 600 rows of W, the first and the last ones among them, are near the
+    hidden states; the other logits are 0, and so are the other rows of gW but for softmax's share of them."""
+    import torch
+    H, V = 2056, 1100003
+    dt = {"s": torch.float32, "b": torch.bfloat16}[prec]
+    gen = torch.Generator("cuda").manual_seed(tokens)
+    W = torch.zeros(V, H, dtype=dt, device="cuda")
+    some = torch.cat([torch.arange(200), torch.arange(V // 2, V // 2 + 200), torch.arange(V - 200, V)])
+    at = some.cuda()
+    W[at] = (torch.randn(600, H, generator=gen, device="cuda") * 0.05).to(dt)
+    pick = torch.randint(0, 600, (tokens,), generator=gen, device="cuda")
+    pick[0], pick[1] = 599, 0
+    label = at[pick].int()
+    X = (torch.randn(tokens, H, generator=gen, device="cuda") + 30 * W[label.long()].float()).to(dt)
+    loss, lse = blas.gpu_xent(prec, H, tokens, V, 1.0, W, H, X, H, label)
+    torch.cuda.synchronize()
+    w64, x64, y = W[at].double().cpu().numpy(), X.double().cpu().numpy(), pick.cpu().numpy()
+    # the reference in 64 bits: the rows of zeros add exp(0) each to the sum and nothing to the products
+    z = x64 @ w64.T
+    top = np.maximum(z.max(axis=1), 0)
+    want = top + np.log(np.exp(z - top[:, None]).sum(axis=1) + (V - 600) * np.exp(-top))
+    dz = (H + 2) * xent_ref.U * (np.abs(x64) @ np.abs(w64).T)
+    # the bound of the reference, with the tiles of all of V
+    blse = dz.max(axis=1) + (128 + 8 + -(-V // 128) + 4) * xent_ref.U + 4 * xent_ref.U * np.abs(want)
+    got = lse.double().cpu().numpy()
+    assert (np.abs(got - want) <= blse).all(), np.abs(got - want) / blse
+    wloss, k = want - z[np.arange(tokens), y], np.arange(tokens)
+    assert (np.abs(loss.double().cpu().numpy() - wloss) <= blse + dz[k, y] + 2 * xent_ref.U * np.abs(wloss)).all()
+    gloss = torch.randn(tokens, generator=gen, device="cuda")
+    gW, gX = torch.full((V, H), float("nan"), dtype=dt, device="cuda"), torch.full_like(X, float("nan"))
+    blas.gpu_xent_grad(prec, H, tokens, V, 1.0, W, H, X, H, label, IGNORE, lse, gloss, None, 0.0, gW, H, gX, H)
+    torch.cuda.synchronize()
+    g64 = gloss.double().cpu().numpy()
+    wW, wX, bW, bX = xent_ref.backward(w64, x64, y, 1.0, IGNORE, got, g64, None, prec)
+    assert (np.abs(gW[at].double().cpu().numpy() - wW) <= bW).all()
+    # sums over V terms, all but 600 of them 0 (an addition of 0 rounds nothing)
+    assert (np.abs(gX.double().cpu().numpy() - wX) <= bX).all()
+    # the rows between: one value a column, sum_t gloss_t exp(-lse_t) x_t
+    share = (g64 * np.exp(-got)) @ x64
+    size = (np.abs(g64) * np.exp(-got)) @ np.abs(x64)
+    v = xent_ref.half_step(prec)
+    # P: 8 u and 2 u |lse| of itself and its rounding; the sum; the result's rounding
+    e = size * ((8 + 4 * np.abs(got).max() + tokens + 8) * xent_ref.U + v)
+    bound = torch.from_numpy(e + v * (np.abs(share) + e) + 2.0 ** -126).cuda()
+    share = torch.from_numpy(share).cuda()
+    for a, b in ((200, V // 2), (V // 2 + 200, V - 200)):
+        for r in range(a, b, 1 << 16):
+            assert ((gW[r:min(r + (1 << 16), b)].double() - share).abs() <= bound).all(), r

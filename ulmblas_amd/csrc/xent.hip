@@ -274,7 +274,8 @@ gx_kernel(int hidden, const int *__restrict__ place, const int *__restrict__ cou
 // sizes
 // ---------------------------------------------------------------------------
 
-constexpr int kMaxHidden = 1 << 20, kMaxRows = 1 << 28, kMaxLd = (1 << 21) - 1;
+// A launch has fewer than 2^32 threads, and some have a workgroup of 256 for each token.
+constexpr int kMaxHidden = 1 << 20, kMaxTokens = 1 << 23, kMaxVocab = 1 << 28, kMaxLd = (1 << 21) - 1;
 
 // testing: at most this many vocabulary rows in a piece (0: by size)
 std::atomic<int> g_piece_rows{0};
@@ -283,7 +284,7 @@ inline int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; 
 
 bool sizes_ok(int hidden, int tokens, int vocab)
 {
-    return hidden >= 1 && hidden <= kMaxHidden && tokens >= 0 && tokens <= kMaxRows && vocab >= 1 && vocab <= kMaxRows;
+    return hidden >= 1 && hidden <= kMaxHidden && tokens >= 0 && tokens <= kMaxTokens && vocab >= 1 && vocab <= kMaxVocab;
 }
 
 // ---------------------------------------------------------------------------
@@ -305,7 +306,7 @@ int launch_tile(const ProductArgs &g, hipStream_t stream)
         if (dev < 32) ready.fetch_or(1u << dev);
     }
     const int64_t tiles = (int64_t)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN);
-    if (tiles > 1 << 30) {
+    if (std::max<int64_t>(tiles, g.groups) * WM * WN * 64 >> 32) {
         g_last_error = "too many tiles for one launch";
         return ULMBLAS_GPU_BAD_ARGUMENT;
     }
@@ -536,7 +537,9 @@ int xent_device(int hidden, int tokens, int vocab, float alpha, const T *W, int 
     g.ldStats = l.tokens_p;
     g.target = part_of<float>(work, l.target);
     const bool direct = in_place(W, ldW, tokens), words = !direct || on_words(W, ldW);
-    const int piece = direct ? vocab : l.piece;
+    // as many rows at a time as one launch has tiles for (128 x 64 ones, 256 threads each)
+    const int64_t most = tokens <= kNarrow ? kMaxVocab : ((int64_t)1 << 36) / tokens / 256 * 256;
+    const int piece = (int)std::min<int64_t>(direct ? vocab : l.piece, most);
     int tiles = 0;
     for (int v0 = 0; v0 < vocab; v0 += piece) {
         g.M = std::min(piece, vocab - v0);
