@@ -17,8 +17,8 @@
 // 118 us, which the bytes of W and gW bound (4.5 - 5.0 TB/s), 8 tokens 165 - 175 us, bound by
 // the 24 multiplications and additions an element of W and their operands' conversion;
 // fp32 205 - 233 us.  The three products as such take 230 and 415 us.  5 x 1001 x 30001
-// bf16: 43 us (70 us by the products), 36 of them in this pass: rows off their alignment,
-// and W read at half of memory's rate.  A kernel for each count of tokens: with values
+// bf16: 43 us (70 us by the products), 36 of them in this pass, which moves 141 MB, 20 of
+// them partial sums of gX (3.9 TB/s).  A kernel for each count of tokens: with values
 // for the next power of two computed too, that pass took 46 us.
 // The exchange between lanes goes through swaps and DPP: through LDS it was the
 // longest part of the work on a set of rows (2 tokens, hidden 1024: 83 -> 34 us).
