@@ -105,6 +105,11 @@ def test_refusals_of_the_group():
     for kw in (dict(largest=-1.0), dict(largest=float("nan")), dict(y=None), dict(y=(4098, 4096)), dict(y=(None, 4096))):
         assert group(which="clip", **kw) == BAD, kw
     assert group(which="clip", count=0, norm=None) == 0
+    # what is written overlaps nothing but its own tensor: 4 fp32 and 4 bf16 elements are 16 and 8 bytes
+    for kw in (dict(y=(4096, 4096)), dict(x=(4096, 4200), y=(4096, 4108)), dict(x=(4096, 4200), y=(4300, 4110)),
+               dict(x=(4096, 4200), y=(4100, 4200)), dict(x=(4096, 4200), y=(4196, 4300))):
+        assert group(which="clip", **kw) == BAD, kw
+        assert b"overlaps" in lib.load().ulmblas_gpu_last_error(), kw
 
 
 def test_wrappers_refuse_what_does_not_fit():

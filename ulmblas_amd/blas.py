@@ -605,34 +605,6 @@ class TensorGroup:
         self.types = b"".join(kinds[x.dtype] for x in self.tensors)
         self.lengths = (C.c_long * max(n, 1))(*[x.numel() for x in self.tensors])
         self.pointers = (C.c_void_p * max(n, 1))(*[x.data_ptr() for x in self.tensors])
-        self._apart = None
-
-    def apart(self):
-        """Whether no two of its tensors overlap."""
-        if self._apart is None:
-            self._apart = _apart(self, self)
-        return self._apart
-
-
-def _apart(read, written):
-    """Whether the tensors of the group `written` overlap neither each other nor any of `read`, but for the one with
-    the same number, which may be the same memory."""
-    spans = []
-    for i, (r, w) in enumerate(zip(read.tensors, written.tensors)):
-        size, start = w.numel() * w.element_size(), w.data_ptr()
-        if size == 0:
-            continue
-        spans.append((start, start + size, True))
-        if r.data_ptr() != start:
-            spans.append((r.data_ptr(), r.data_ptr() + size, False))
-    spans.sort()
-    end = end_written = 0
-    for start, stop, writes in spans:
-        if start < (end if writes else end_written):
-            return False
-        end = max(end, stop)
-        end_written = max(end_written, stop) if writes else end_written
-    return True
 
 
 def _as_group(tensors):
@@ -668,8 +640,6 @@ def gpu_gclip(tensors, dNorm, largest, out=None, stream=None):
     o = g if out is None else _as_group(out)
     if o.types != g.types or list(o.lengths) != list(g.lengths):
         raise ValueError("out: lengths and types must be those of the tensors")
-    if not (g.apart() if o is g else _apart(g, o)):
-        raise ValueError("a tensor that is written overlaps another one")
     _vector("norm", dNorm, 1, torch.float32)
     device = _device_of((("tensors", g.tensors[0] if g.count else None), ("out", o.tensors[0] if o.count else None),
                          ("norm", dNorm)))
