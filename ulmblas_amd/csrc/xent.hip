@@ -20,7 +20,6 @@
 #include "xent_kernel.hip.h"
 
 #include <algorithm>
-#include <cstdio>
 
 using namespace ulmgpu;
 using namespace ulmgpu::xent;

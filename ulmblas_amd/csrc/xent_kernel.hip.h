@@ -32,7 +32,7 @@
 // 4096 x 8192 x 65536, in blocks 3.32 ms).
 //
 // Measured on bf16 tiles of 256 x 256, K = 65536 (GX) and 4096 (STATS): the
-// matrix cores are busy 70 % of the time at the 1.8 - 2.1 GHz that the power
+// matrix cores are busy 57 - 70 % of the time at the 1.8 - 2.1 GHz that the power
 // limit leaves.  With the fetches left out the same loop runs 25 % faster,
 // with all of them served by L2 10 % faster; more steps in flight (up to 2) do
 // not help.  16 x 16 MFMAs run at a higher clock than 32 x 32 ones (they read
@@ -44,7 +44,6 @@
 
 #include <cmath>
 #include <cstdint>
-#include <type_traits>
 
 namespace ulmgpu {
 namespace xent {
@@ -55,7 +54,6 @@ typedef __attribute__((ext_vector_type(4))) short vshort4;
 typedef __attribute__((ext_vector_type(8))) short vshort8;
 typedef __attribute__((ext_vector_type(8))) __bf16 vbf8;
 typedef __attribute__((ext_vector_type(4))) float vfloat4;
-typedef __attribute__((ext_vector_type(16))) float vfloat16;
 
 // bf16 values are carried as their bits.
 using bf16_t = unsigned short;
