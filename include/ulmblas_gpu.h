@@ -620,9 +620,10 @@ int ulmblas_gpu_set_variant(int precision /* 'd' or 's' */, int variant);
  *                     any-shape kernel alone over the triangle; 4, 5: as 1, 2
  *                     with the second largest tile (blocks of its order) for
  *                     the square;
- *  XENT_PIECE         value > 0: the gradient of the cross entropy takes at most
+ *  XENT_PIECE         value > 0: the cross entropy and its gradient take at most
  *                     this many columns of W (rounded up to 256) at a time; 0
- *                     (default): as many as the workspace's bound allows;
+ *                     (default): as many as the workspace's bound and a
+ *                     launch allow;
  *  FAIL_ALLOC         the next `value` device allocations of the host entry
  *                     points fail (as if the device were out of memory).
  * Every kernel runs to its end whatever is set here. */

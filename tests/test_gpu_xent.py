@@ -439,3 +439,27 @@ def test_classifier_past_32_bits(prec, tokens):
     for a, b in ((200, V // 2), (V // 2 + 200, V - 200)):
         for r in range(a, b, 1 << 16):
             assert ((gW[r:min(r + (1 << 16), b)].double() - share).abs() <= bound).all(), r
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+def test_more_tiles_than_a_launch_takes(prec):
+    """Tokens times vocabulary beyond 2^36: the forward product goes out in several launches (here two, from row 32512
+    on).  Half of the labels and most of the softmax are in the rows of the second one."""
+    import torch
+    H, T, V = 8, (1 << 21) + 3, 33000
+    dt = {"s": torch.float32, "b": torch.bfloat16}[prec]
+    gen = torch.Generator("cuda").manual_seed(7)
+    X = torch.randn(T, H, generator=gen, device="cuda").to(dt)
+    W = torch.randn(V, H, generator=gen, device="cuda")
+    W[32512:] *= 3.0
+    W = W.to(dt)
+    label = torch.randint(0, V, (T,), generator=gen, device="cuda", dtype=torch.int32)
+    label[::2] = torch.randint(32512, V, ((T + 1) // 2,), generator=gen, device="cuda", dtype=torch.int32)
+    loss, lse = blas.gpu_xent(prec, H, T, V, 1.0, W, H, X, H, label)
+    torch.cuda.synchronize()
+    at = torch.cat([torch.arange(200), torch.arange(T // 2 - 100, T // 2 + 100), torch.arange(T - 200, T)]).cuda()
+    w64, x64, y = W.double().cpu().numpy(), X[at].double().cpu().numpy(), label[at].cpu().numpy()
+    wloss, wlse, blse, bloss = xent_ref.forward(w64, x64, y, 1.0, IGNORE, prec)
+    off = [float((np.abs(got[at].double().cpu().numpy() - want) / bound).max())
+           for got, want, bound in ((lse, wlse, blse), (loss, wloss, bloss))]
+    assert max(off) <= 1, off

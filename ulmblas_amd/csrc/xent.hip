@@ -537,14 +537,15 @@ int xent_device(int hidden, int tokens, int vocab, float alpha, const T *W, int 
     g.target = part_of<float>(work, l.target);
     const bool direct = in_place(W, ldW, tokens), words = !direct || on_words(W, ldW);
     // as many rows at a time as one launch has tiles for (128 x 64 ones, 256 threads each)
-    const int64_t most = tokens <= kNarrow ? kMaxVocab : ((int64_t)1 << 36) / tokens / 256 * 256;
+    int64_t most = tokens <= kNarrow ? kMaxVocab : ((int64_t)1 << 36) / tokens / 256 * 256;
+    if (g_piece_rows.load() > 0) most = std::min<int64_t>(most, round_up(g_piece_rows.load(), 256));
     const int piece = (int)std::min<int64_t>(direct ? vocab : l.piece, most);
     int tiles = 0;
     for (int v0 = 0; v0 < vocab; v0 += piece) {
         g.M = std::min(piece, vocab - v0);
         g.first = v0;
         if (direct) {
-            g.A = W;
+            g.A = W + (int64_t)v0 * ldW;
             g.ldA = (int64_t)ldW * sizeof(T);
             g.widthA = hidden;
         } else {
