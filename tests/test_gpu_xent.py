@@ -463,3 +463,102 @@ def test_more_tiles_than_a_launch_takes(prec):
     off = [float((np.abs(got[at].double().cpu().numpy() - want) / bound).max())
            for got, want, bound in ((lse, wlse, blse), (loss, wloss, bloss))]
     assert max(off) <= 1, off
+
+
+def busy():
+    """Tens of milliseconds of work on the current stream."""
+    import torch
+    a = torch.ones(8192, 8192, device="cuda")
+    for _ in range(4):
+        a = a @ a * 2.0 ** -13
+    return a
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+@pytest.mark.parametrize("tokens", [4, 300])
+@pytest.mark.parametrize("to_default", [False, True])
+def test_another_stream_comes_after_the_current_one(prec, tokens, to_default):
+    """Operands and workspaces that the current stream is still filling, and new memory whose last user is still at
+    work there: a call on another stream comes after both."""
+    import torch
+    p = Problem(prec, 264, tokens, 3000, seed=41, masked=0.2)
+    H, T, V = p.H, p.T, p.V
+    f = [torch.from_numpy(a).cuda() for a in (p.gloss, p.glse)]
+    X, label = p.X.contiguous(), p.dlabel
+    sizes = [blas.xent_worksize(prec, H, T, V), blas.xent_grad_worksize(prec, H, T, V)]
+
+    def step(X, label, out, works, stream):
+        loss, lse = blas.gpu_xent(prec, H, T, V, 1.0, p.W, p.ldW, X, H, label, IGNORE, *out[:2], work=works[0], stream=stream)
+        gW, gX = blas.gpu_xent_grad(prec, H, T, V, 1.0, p.W, p.ldW, X, H, label, IGNORE, lse, *f, 0.0, out[2], H, out[3], H,
+                                    work=works[1], stream=stream)
+        norm = blas.gpu_gnrm2([gW, gX], out[4], work=works[2], stream=stream)
+        blas.gpu_gclip([gW, gX], norm, 0.5 * scale, stream=stream)
+        return [loss, lse, gW, gX, norm]
+
+    def fresh():
+        return [None, None, torch.empty(V, H, dtype=X.dtype, device="cuda"),
+                torch.empty(T, H, dtype=X.dtype, device="cuda"), None]
+
+    scale = 1.0
+    scale = float(step(X, label, fresh(), [None] * 3, None)[4])
+    want = step(X, label, fresh(), [None] * 3, None)
+    torch.cuda.synchronize()
+    first, second = torch.cuda.current_stream(), torch.cuda.Stream()
+    current, other = (second, first) if to_default else (first, second)
+    with torch.cuda.stream(current):
+        for given in (True, False):
+            late_x, late_label = torch.full_like(X, float("nan")), torch.full_like(label, IGNORE)
+            out, works = fresh(), [None] * 3
+            torch.cuda.synchronize()
+            busy()
+            late_x.copy_(X)
+            late_label.copy_(label)
+            if given:
+                out = [torch.full_like(x, float("nan")) for x in want]
+                works = [p.work(n) for n in sizes] + [p.work(blas.gnrm2_worksize(want[2:4]))]
+            else:               # memory of these sizes goes back to the allocator while it is still to be written
+                for n in sizes + [4 * T] * 2 + [blas.gnrm2_worksize(want[2:4])]:
+                    p.work(n)
+            got = step(late_x, late_label, out, works, other.cuda_stream)
+            other.synchronize()
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+            torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+def test_another_stream_inside_a_capture(prec):
+    """A second stream of the same capture, with and without new memory; a stream outside gets no new memory."""
+    import torch
+    p = Problem(prec, 264, 70, 3000, seed=42, masked=0.2)
+    H, T, V = p.H, p.T, p.V
+    X, label = p.X.contiguous(), p.dlabel
+    loss, lse = torch.empty(T, device="cuda"), torch.empty(T, device="cuda")
+    work = p.work(blas.xent_worksize(prec, H, T, V))
+    side, outside = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def call(stream, *given, work=None):
+        return blas.gpu_xent(prec, H, T, V, 1.0, p.W, p.ldW, X, H, label, IGNORE, *given, work=work, stream=stream)
+
+    call(None, loss, lse, work=work)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        side.wait_stream(torch.cuda.current_stream())
+        call(side.cuda_stream, loss, lse, work=work)
+        loss2, lse2 = call(side.cuda_stream)
+        with pytest.raises(ValueError, match="captured"):
+            call(outside.cuda_stream)
+        torch.cuda.current_stream().wait_stream(side)
+        total = loss + loss2
+    for seed in range(4):
+        label.copy_(torch.randint(0, V, (T,), device="cuda"))
+        X.copy_(torch.randn(T, H, device="cuda"))
+        wloss, wlse = call(None)
+        torch.cuda.synchronize()
+        for x in (loss, lse, loss2, lse2, total):
+            x.fill_(float("nan"))
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in ((loss, wloss), (lse, wlse), (loss2, wloss), (lse2, wlse), (total, 2 * wloss)):
+            assert torch.equal(a, b), seed

@@ -139,3 +139,80 @@ def test_wrappers_refuse_what_does_not_fit():
         blas.TensorGroup([torch.zeros(4, 4).T])
     with pytest.raises(ValueError, match="not on a GPU"):
         blas.TensorGroup([f])
+
+
+class FakeStreams:
+    """torch's streams and allocator as far as the wrappers use them: a log of what they do, in order."""
+
+    def __init__(self, monkeypatch, captured=()):
+        torch = pytest.importorskip("torch")
+        self.log, self.now, fake = [], 7, self
+
+        class Stream:
+            def __init__(self, raw, device=None):
+                self.cuda_stream = raw or "a new one"
+
+            def wait_stream(self, other):
+                fake.log.append(f"{self.cuda_stream} waits for {other.cuda_stream}")
+
+        default = Stream(1)
+        default.cuda_stream = 0
+
+        class Inside:
+            def __init__(self, stream):
+                self.stream = stream
+
+            def __enter__(self):
+                self.before, fake.now = fake.now, self.stream.cuda_stream
+
+            def __exit__(self, *exc):
+                fake.now = self.before
+
+        class Tensor:
+            def record_stream(self, stream):
+                fake.log.append(f"kept for {stream.cuda_stream}")
+
+        def empty(n, **kw):
+            fake.log.append(f"memory of {fake.now}")
+            return Tensor()
+
+        for name, value in (("current_device", lambda: 0), ("current_stream", lambda *a: Stream(fake.now)),
+                            ("ExternalStream", Stream), ("default_stream", lambda *a: default), ("stream", Inside),
+                            ("is_current_stream_capturing", lambda: fake.now in captured)):
+            monkeypatch.setattr(torch.cuda, name, value)
+        monkeypatch.setattr(torch, "empty", empty)
+        self.device = torch.device("cuda", 0)
+        self.dtype = torch.uint8
+
+
+def test_another_stream_waits_before_memory_is_handed_out(monkeypatch):
+    """The allocator hands out memory in the current stream's order: another stream has to wait for that one first."""
+    f = FakeStreams(monkeypatch)
+    with blas._On(f.device, 11) as on:
+        assert on.stream == 11
+        on.empty(5, f.dtype)
+    assert f.log == ["11 waits for 7", "memory of 7", "kept for 11"]
+    f.log.clear()
+    with blas._On(f.device, 0) as on:           # the default stream
+        assert on.stream == 0
+        on.empty(5, f.dtype)
+    assert f.log == ["0 waits for 7", "memory of 7", "kept for 0"]
+    for given in (None, 7):
+        f.log.clear()
+        with blas._On(f.device, given) as on:
+            assert on.stream == 7
+            on.empty(5, f.dtype)
+        assert f.log == ["memory of 7"]
+
+
+@pytest.mark.parametrize("captured", [(7,), (11,), (7, 11)])
+def test_another_stream_of_a_capture(monkeypatch, captured):
+    f = FakeStreams(monkeypatch, captured)
+    with blas._On(f.device, 11) as on:
+        if len(captured) == 2:
+            on.empty(5, f.dtype)
+            assert f.log == ["11 waits for 7", "memory of 7", "kept for 11"]
+        else:                           # nothing can wait across a capture's border: no new memory, no order
+            with pytest.raises(ValueError, match="captured"):
+                on.empty(5, f.dtype)
+            assert f.log == [] and on.stream == 11

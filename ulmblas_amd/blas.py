@@ -462,21 +462,46 @@ def _device_of(named):
 
 
 class _On:
-    """The operands' device as the current one, with the stream to enqueue on (a raw
-    hipStream_t value, or None: torch's current stream of that device)."""
+    """The operands' device as the current one, with the stream to enqueue on: a raw hipStream_t value, or None for
+    torch's current stream of that device.
+
+    A stream other than the current one waits for what is enqueued there so far: operands that torch is still filling,
+    and new memory, which the allocator hands out in the current stream's order while its last user may be at work.
+    (A call that is to run beside that work is made inside torch.cuda.stream(...) instead.)  Between a stream that is
+    being captured and one that is not nothing can wait, so such a call gets no new memory either."""
 
     def __init__(self, device, stream):
         import torch
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
         self._given, self._device = stream, device
+        self._other, self._apart = None, False
         self._guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
     def __enter__(self):
-        import torch
         if self._guard is not None:
             self._guard.__enter__()
-        self.stream = torch.cuda.current_stream().cuda_stream if self._given is None else self._given
+        try:
+            self._order()
+        except BaseException:
+            self.__exit__(None, None, None)
+            raise
         return self
+
+    def _order(self):
+        import torch
+        current = torch.cuda.current_stream()
+        self.stream = current.cuda_stream if self._given is None else self._given
+        if self.stream == current.cuda_stream:
+            return
+        # 0 is the default stream, for which ExternalStream(0) would stand for a new one
+        other = (torch.cuda.ExternalStream(self.stream, device=self._device) if self.stream else
+                 torch.cuda.default_stream(self._device))
+        captured = torch.cuda.is_current_stream_capturing()
+        with torch.cuda.stream(other):
+            self._apart = captured != torch.cuda.is_current_stream_capturing()
+        if not self._apart:
+            other.wait_stream(current)
+            self._other = other
 
     def __exit__(self, *exc):
         if self._guard is not None:
@@ -485,9 +510,12 @@ class _On:
     def empty(self, n, dtype):
         """A new tensor whose memory is not handed out again before the work on the stream is done."""
         import torch
+        if self._apart:
+            raise ValueError("results and workspace have to be given where only one of the current stream and the "
+                             "stream of the call is being captured")
         x = torch.empty(n, dtype=dtype, device=self._device)
-        if self._given is not None:
-            x.record_stream(torch.cuda.ExternalStream(self._given, device=self._device))
+        if self._other is not None:
+            x.record_stream(self._other)
         return x
 
     def workspace(self, work, size):
@@ -542,7 +570,7 @@ def gpu_xent(prec, hidden, tokens, vocab, alpha, dW, ldW, dX, ldX, dLabel, ignor
     bfloat16 operands).  dW holds the classifier as a column-major hidden x vocab window (a torch [vocab, hidden]
     matrix with row stride ldW), dX the hidden states likewise, dLabel int32 labels; tokens whose label is `ignore`
     or no row of the classifier have loss and lse 0.  Returns (dLoss, dLse), float32, allocated unless given.
-    Asynchronous."""
+    Asynchronous; a `stream` (raw hipStream_t value) other than torch's current one waits for the current one first."""
     import torch
     _window("W", prec, dW, hidden, vocab, ldW)
     _window("X", prec, dX, hidden, tokens, ldX)
@@ -565,7 +593,7 @@ def gpu_xent_grad(prec, hidden, tokens, vocab, alpha, dW, ldW, dX, ldX, dLabel, 
                   ldGW, dGX, ldGX, work=None, stream=None):
     """Gradient of gpu_xent: dLse is its second result, dGLoss and dGLse (None: zero) the gradients of its results.
     dGX (hidden x tokens) and dGW (hidden x vocab, alpha * X * P^T + beta * dGW) take the operands' type; None leaves
-    one out.  Returns (dGW, dGX).  Asynchronous."""
+    one out.  Returns (dGW, dGX).  Asynchronous; `stream` as for gpu_xent."""
     import torch
     for name, x, cols, ld in (("W", dW, vocab, ldW), ("X", dX, tokens, ldX), ("gW", dGW, vocab, ldGW),
                               ("gX", dGX, tokens, ldGX)):
@@ -618,7 +646,7 @@ def gnrm2_worksize(tensors):
 
 def gpu_gnrm2(tensors, dNorm=None, work=None, stream=None):
     """Euclidean norm of a TensorGroup (or list of tensors) taken as one vector, into the float32 device tensor
-    dNorm (one element, allocated unless given), which is returned.  Asynchronous."""
+    dNorm (one element, allocated unless given), which is returned.  Asynchronous; `stream` as for gpu_xent."""
     import torch
     g = _as_group(tensors)
     device = _device_of((("tensors", g.tensors[0] if g.count else None), ("norm", dNorm), ("work", work)))
@@ -634,7 +662,7 @@ def gpu_gnrm2(tensors, dNorm=None, work=None, stream=None):
 def gpu_gclip(tensors, dNorm, largest, out=None, stream=None):
     """Multiplies a TensorGroup (or list of tensors) by min(1, largest / dNorm), in place or into the TensorGroup (or
     list) `out` of the same lengths and types; returns the group that was written.  No tensor that is written may
-    overlap another one (a group of the same tensor twice is refused).  Asynchronous."""
+    overlap another one (a group of the same tensor twice is refused).  Asynchronous; `stream` as for gpu_xent."""
     import torch
     g = _as_group(tensors)
     o = g if out is None else _as_group(out)
