@@ -388,3 +388,23 @@ def test_more_rows_than_the_panel_kernel_holds(oracle):
     assert np.array_equal(got[m:], A0[m:]), "padding rows were written"
     check_factors(A0, got, piv, m, n, (m, n))
     assert np.abs(got[:m] - want[:m]).max() <= 1e-9 * np.abs(want[:m]).max()
+
+
+def test_factorisation_on_another_stream_comes_after_the_current_one():
+    """The matrix, the pivots and the workspace are still being filled on the current stream when the factorisation is
+    enqueued on another one."""
+    import torch
+    n = 700
+    dA = to_device(synth.matrix(85, n, n, n))
+    want = dA.clone()
+    wPiv, wInfo = blas.gpu_dgetrf(n, n, want, n)
+    s = torch.cuda.Stream()
+    late = torch.full_like(dA, float("nan"))
+    torch.cuda.synchronize()
+    a = torch.ones(8192, 8192, device="cuda")
+    for _ in range(4):
+        a = a @ a * 2.0 ** -13
+    late.copy_(dA)
+    dPiv, dInfo = blas.gpu_dgetrf(n, n, late, n, stream=s.cuda_stream)
+    s.synchronize()
+    assert int(dInfo[0]) == 0 == int(wInfo[0]) and torch.equal(dPiv, wPiv) and torch.equal(late, want)

@@ -172,6 +172,9 @@ class FakeStreams:
             def record_stream(self, stream):
                 fake.log.append(f"kept for {stream.cuda_stream}")
 
+            def __getitem__(self, key):
+                return self
+
         def empty(n, **kw):
             fake.log.append(f"memory of {fake.now}")
             return Tensor()
@@ -181,6 +184,7 @@ class FakeStreams:
                             ("is_current_stream_capturing", lambda: fake.now in captured)):
             monkeypatch.setattr(torch.cuda, name, value)
         monkeypatch.setattr(torch, "empty", empty)
+        monkeypatch.setattr(torch, "zeros", empty)
         self.device = torch.device("cuda", 0)
         self.dtype = torch.uint8
 
@@ -215,4 +219,26 @@ def test_another_stream_of_a_capture(monkeypatch, captured):
         else:                           # nothing can wait across a capture's border: no new memory, no order
             with pytest.raises(ValueError, match="captured"):
                 on.empty(5, f.dtype)
-            assert f.log == [] and on.stream == 11
+            assert f.log == ["memory of 7"] and on.stream == 11
+
+
+def test_another_stream_of_the_other_calls_with_new_memory(monkeypatch):
+    """LU and the complex product: pivots, status and workspace are filled and handed out before the stream waits."""
+    torch = pytest.importorskip("torch")
+    A = torch.zeros(8, 8, dtype=torch.float64)
+    f = FakeStreams(monkeypatch)
+
+    class Library:
+        def __getattr__(self, name):
+            if name.endswith("worksize"):
+                return lambda *a: 64
+            return lambda *a: f.log.append(f"{name} on {a[-1]}") or 0
+
+    library = Library()
+    monkeypatch.setattr(blas, "load", lambda: library)
+    monkeypatch.setattr(blas, "_dev_ptr", lambda x: None)
+    blas.gpu_dgetrf(8, 8, A, 8, stream=11)
+    assert f.log == ["memory of 7"] * 3 + ["11 waits for 7"] + ["kept for 11"] * 3 + ["ulmblas_gpu_dgetrf on 11"]
+    f.log.clear()
+    blas.gpu_cgemm("z", "N", "N", 2, 2, 2, 1.0, A, 2, A, 2, 0.0, A, 2, stream=11)
+    assert f.log == ["memory of 7", "11 waits for 7", "kept for 11", "ulmblas_gpu_zgemm on 11"]

@@ -392,20 +392,24 @@ def gpu_symm(prec, right, lower, m, n, alpha, dA, ldA, dB, ldB, beta, dC, ldC, w
 def gpu_cgemm(prec, transA, transB, m, n, k, alpha, dA, ldA, dB, ldB, beta, dC, ldC, stream=None, work=None):
     """Device-resident complex GEMM on torch CUDA tensors (complex dtype, column-major
     windows); transA / transB are characters N, T, C, R.  Allocates the workspace unless
-    one is passed.  Asynchronous; returns (dC, work)."""
+    one is passed.  Asynchronous; returns (dC, work); `stream` as for gpu_xent."""
     import torch
     L = load()
     tb = TRANS_OF_CHAR[transB.upper()]
+    new = []
     if work is None:
         size = getattr(L, f"ulmblas_gpu_{prec}gemm_worksize")(tb, m, n, k)
         work = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda")
+        new.append(work)
     al, be = _pair(alpha, prec), _pair(beta, prec)
     _fits("A", prec, dA, *((m, k) if transA.upper() in "NR" else (k, m)), ldA)
     _fits("B", prec, dB, *((k, n) if transB.upper() in "NR" else (n, k)), ldB)
     _fits("C", prec, dC, m, n, ldC)
-    _status(getattr(L, f"ulmblas_gpu_{prec}gemm")(TRANS_OF_CHAR[transA.upper()], tb, m, n, k, _p(al), _dev_ptr(dA), ldA,
-                                                  _dev_ptr(dB), ldB, _p(be), _dev_ptr(dC), ldC, _dev_ptr(work),
-                                                  _stream(stream)))
+    with _On(None, stream) as on:
+        on.keep(*new)
+        _status(getattr(L, f"ulmblas_gpu_{prec}gemm")(TRANS_OF_CHAR[transA.upper()], tb, m, n, k, _p(al), _dev_ptr(dA),
+                                                      ldA, _dev_ptr(dB), ldB, _p(be), _dev_ptr(dC), ldC, _dev_ptr(work),
+                                                      on.stream))
     return dC, work
 
 
@@ -413,19 +417,21 @@ def gpu_dgetrf(m, n, dA, ldA, stream=None, work=None):
     """Device-resident LU on a torch CUDA tensor holding the column-major
     window.  Returns (dPiv, dInfo) as int32 device tensors; asynchronous.
     `work`: a caller's workspace of at least ulmblas_gpu_dgetrf_worksize()
-    bytes (any contents; one factorisation at a time may use it)."""
+    bytes (any contents; one factorisation at a time may use it); `stream` as for gpu_xent."""
     import torch
     _fits("A", "d", dA, m, n, ldA)
-    s = torch.cuda.current_stream().cuda_stream if stream is None else stream
     L = load()
     dPiv = torch.zeros(max(min(m, n), 1), dtype=torch.int32, device="cuda")
     dInfo = torch.zeros(1, dtype=torch.int32, device="cuda")
+    new = [dPiv, dInfo]
     if work is None:
         work = torch.zeros((L.ulmblas_gpu_dgetrf_worksize() + 7) // 8, dtype=torch.float64, device="cuda")
+        new.append(work)
     elif work.numel() * work.element_size() < L.ulmblas_gpu_dgetrf_worksize():
         raise ValueError("workspace smaller than ulmblas_gpu_dgetrf_worksize()")
-    _status(L.ulmblas_gpu_dgetrf(m, n, _dev_ptr(dA), ldA, _dev_ptr(dPiv), _dev_ptr(dInfo), _dev_ptr(work),
-                                 C.c_void_p(s)))
+    with _On(None, stream) as on:           # after the fills: another stream waits for them
+        on.keep(*new)
+        _status(L.ulmblas_gpu_dgetrf(m, n, _dev_ptr(dA), ldA, _dev_ptr(dPiv), _dev_ptr(dInfo), _dev_ptr(work), on.stream))
     dInfo._ulm_work = work          # keep the workspace alive until the results are read
     return dPiv[:min(m, n)], dInfo
 
@@ -507,15 +513,19 @@ class _On:
         if self._guard is not None:
             self._guard.__exit__(*exc)
 
-    def empty(self, n, dtype):
-        """A new tensor whose memory is not handed out again before the work on the stream is done."""
-        import torch
-        if self._apart:
+    def keep(self, *new):
+        """New tensors: their memory is not handed out again before the work on the stream is done."""
+        if new and self._apart:
             raise ValueError("results and workspace have to be given where only one of the current stream and the "
                              "stream of the call is being captured")
-        x = torch.empty(n, dtype=dtype, device=self._device)
         if self._other is not None:
-            x.record_stream(self._other)
+            for x in new:
+                x.record_stream(self._other)
+
+    def empty(self, n, dtype):
+        import torch
+        x = torch.empty(n, dtype=dtype, device=self._device)
+        self.keep(x)
         return x
 
     def workspace(self, work, size):
