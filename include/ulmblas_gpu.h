@@ -507,7 +507,8 @@ int ulmblas_gpu_dlaswp(int n, double *dA, int ldA, int k1, int k2,
  * ulmblas_gpu_?xent_worksize(hidden, tokens, vocab) bytes, 16-byte aligned, any
  * contents, for one call at a time.  hidden at most 2^20, tokens at most 2^23,
  * vocab at most 2^28 (worksize 0, BAD_ARGUMENT beyond that), ldW below 2^21;
- * tokens == 0 does nothing.
+ * tokens == 0 does nothing.  dLoss, dLse and `work` share no memory with each
+ * other or the operands (BAD_ARGUMENT).
  * Everything is enqueued on `stream`, on the current device; nothing is
  * allocated or synchronised.  The same call gives the same bits. */
 long ulmblas_gpu_sxent_worksize(int hidden, int tokens, int vocab);
@@ -530,8 +531,10 @@ int ulmblas_gpu_bxent(int hidden, int tokens, int vocab, float alpha,
  * beta == 0 never reads gW.  A null dGW or dGX is not computed.  The logits are
  * computed again, a piece of the vocabulary at a time, and P of that piece is
  * rounded to the operands' type for the two products (up to 8 tokens it is not:
- * hidden up to 4096, or 8192 with up to 4 tokens).  Outputs must not overlap
- * inputs, each other or `work` (ulmblas_gpu_?xent_grad_worksize bytes). */
+ * hidden up to 4096, or 8192 with up to 4 tokens).  dGW, dGX and `work`
+ * (ulmblas_gpu_?xent_grad_worksize bytes) share no memory with each other or
+ * the operands (BAD_ARGUMENT); the columns of one matrix may lie between those
+ * of another. */
 long ulmblas_gpu_sxent_grad_worksize(int hidden, int tokens, int vocab);
 long ulmblas_gpu_bxent_grad_worksize(int hidden, int tokens, int vocab);
 int ulmblas_gpu_sxent_grad(int hidden, int tokens, int vocab, float alpha,

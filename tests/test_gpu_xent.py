@@ -562,3 +562,32 @@ def test_another_stream_inside_a_capture(prec):
         torch.cuda.synchronize()
         for a, b in ((loss, wloss), (lse, wlse), (loss2, wloss), (lse2, wlse), (total, 2 * wloss)):
             assert torch.equal(a, b), seed
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+@pytest.mark.parametrize("tokens", [5, 90])
+def test_gradients_between_the_rows_of_the_operands(prec, tokens):
+    """X beside gX and W beside gW in the halves of wide matrices, loss beside lse: no memory is shared."""
+    import torch
+    p = Problem(prec, 200, tokens, 1300, seed=51, masked=0.2)
+    H, T, V = p.H, p.T, p.V
+    f = [torch.from_numpy(a).cuda() for a in (p.gloss, p.glse)]
+    want = list(blas.gpu_xent(prec, H, T, V, 1.0, p.W, p.ldW, p.X, p.ldX, p.dlabel, IGNORE))
+    gW, gX = torch.empty(V, H, dtype=p.W.dtype, device="cuda"), torch.empty(T, H, dtype=p.W.dtype, device="cuda")
+    want += blas.gpu_xent_grad(prec, H, T, V, 1.0, p.W, p.ldW, p.X, p.ldX, p.dlabel, IGNORE, want[1], *f, 0.0, gW, H, gX, H)
+    wide = torch.zeros(V + 1, 2 * H, dtype=gW.dtype, device="cuda")
+    w, x, both = wide[:V], torch.zeros_like(gX).repeat(1, 3), torch.empty(2 * T, device="cuda")
+    w[:, H:], x[:, H:2 * H] = p.W, p.X
+    got = list(blas.gpu_xent(prec, H, T, V, 1.0, w[:, H:], 2 * H, x[:, H:], 3 * H, p.dlabel, IGNORE, both[:T], both[T:]))
+    got += blas.gpu_xent_grad(prec, H, T, V, 1.0, w[:, H:], 2 * H, x[:, H:], 3 * H, p.dlabel, IGNORE, got[1], *f, 0.0,
+                              w, 2 * H, x, 3 * H)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a[:, :H] if a.dim() == 2 else a, b)
+    assert torch.equal(w[:, H:].float().nan_to_num(), p.W.float().nan_to_num()) and (x[:, 2 * H:] == 0).all()
+    for off in (1, 2 * H - 1):          # one element of every row too far
+        with pytest.raises(blas.GpuError, match="overlaps"):
+            blas.gpu_xent_grad(prec, H, T, V, 1.0, w[:, H:], 2 * H, x[:, H:], 3 * H, p.dlabel, IGNORE, got[1], *f, 0.0,
+                               wide.view(-1)[off:], 2 * H, None, H)
+    with pytest.raises(blas.GpuError, match="overlaps"):
+        blas.gpu_xent(prec, H, T, V, 1.0, p.W, p.ldW, p.X, p.ldX, p.dlabel, IGNORE, both[:T], both[T - 1:2 * T - 1])

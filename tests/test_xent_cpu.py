@@ -242,3 +242,72 @@ def test_another_stream_of_the_other_calls_with_new_memory(monkeypatch):
     f.log.clear()
     blas.gpu_cgemm("z", "N", "N", 2, 2, 2, 1.0, A, 2, A, 2, 0.0, A, 2, stream=11)
     assert f.log == ["memory of 7", "11 waits for 7", "kept for 11", "ulmblas_gpu_zgemm on 11"]
+
+
+def have_gpu():
+    return pytest.importorskip("torch").cuda.is_available()
+
+
+AREA = {name: C.c_void_p((i + 1) << 44) for i, name in enumerate(("W", "X", "label", "loss", "lse", "gloss", "gW", "gX", "work"))}
+
+
+def refused(call, p, **kw):
+    """Whether a call on addresses that nothing follows is refused for an overlap (anything else needs a GPU)."""
+    names = ("W", "X", "label", "loss", "lse", "work") if call is xent else ("W", "X", "label", "lse", "gloss", "gW", "gX", "work")
+    status = call(p, **{**{n: AREA[n] for n in names}, **kw})
+    text = lib.load().ulmblas_gpu_last_error()
+    assert status != 0
+    return status == BAD and b"overlaps" in text
+
+
+@pytest.mark.parametrize("p", ["s", "b"])
+def test_overlapping_operands_are_refused(p):
+    size = {"s": 4, "b": 2}[p]
+
+    def at(name, off):
+        return C.c_void_p(AREA[name].value + off)
+
+    # hidden 8, 4 tokens, 10 columns of W: the last bytes of each operand
+    last = {"W": 80 * size, "X": 32 * size, "label": 16, "loss": 16, "lse": 16, "gloss": 16, "gW": 80 * size, "gX": 32 * size}
+    for a in ("loss", "lse", "work"):
+        for b in ("W", "X", "label", "loss", "lse"):
+            if a != b:
+                assert refused(xent, p, **{a: at(b, 0)}), (a, b)
+                assert refused(xent, p, **{a: at(b, last[b] // 16 * 16 - 16)}), (a, b)
+    assert refused(xent, p, loss=at("work", blas.xent_worksize(p, 8, 4, 10) - 4))
+    for tokens in (4, 16):
+        for a in ("gW", "gX", "work"):
+            for b in ("W", "X", "label", "lse", "gloss", "gW", "gX"):
+                if a != b:
+                    assert refused(grad, p, tokens=tokens, **{a: at(b, 0)}), (a, b)
+                    assert refused(grad, p, tokens=tokens, **{a: at(b, last[b] // 16 * 16 - 16)}), (a, b)
+        assert refused(grad, p, tokens=tokens, gW=at("work", blas.xent_grad_worksize(p, 8, tokens, 10) - 4))
+    # the gradient of lse, too
+    assert lib.load()[f"ulmblas_gpu_{p}xent_grad"](8, 4, 10, C.c_float(1.0), AREA["W"], 8, AREA["X"], 8, AREA["label"], -100,
+                                                   AREA["lse"], AREA["gloss"], AREA["gX"], C.c_float(0.0), AREA["gW"], 8,
+                                                   AREA["gX"], 8, AREA["work"], None) == BAD
+
+
+def test_windows_between_the_columns_of_others():
+    """Random windows in one area: refused exactly where a written one shares an element with another."""
+    if have_gpu():
+        pytest.skip("the calls that are not refused would run on addresses that nothing follows")
+    rng = np.random.default_rng(17)
+    met = 0
+    for trial in range(1500):
+        H, T, V = (int(n) for n in (rng.integers(1, 5), rng.integers(1, 12), rng.integers(1, 12)))
+        pitch = int(rng.integers(H, 12))
+        # half the trials: all columns equally far apart, as in the parts of one wide matrix
+        ld = [pitch if trial % 2 else int(rng.integers(H, 14)) for _ in range(4)]
+        at = [int(rng.integers(0, 60)) for _ in range(4)]
+        if trial % 3 == 0:
+            at = [int(a) * H for a in rng.permutation(4)]
+        columns = (V, T, V, T)
+        cells = [{a + c * l + h for c in range(n) for h in range(H)} for a, l, n in zip(at, ld, columns)]
+        meets = any(cells[i] & cells[j] for i in (2, 3) for j in range(4) if i != j)
+        where = [C.c_void_p(AREA["W"].value + 4 * a) for a in at]
+        got = refused(grad, "s", hidden=H, tokens=T, vocab=V, ldW=ld[0], ldX=ld[1], ldGW=ld[2], ldGX=ld[3], W=where[0],
+                      X=where[1], gW=where[2], gX=where[3])
+        assert got == meets, (H, T, V, ld, at)
+        met += meets
+    assert 200 < met < 1300         # both answers were asked for

@@ -20,6 +20,8 @@
 #include "xent_kernel.hip.h"
 
 #include <algorithm>
+#include <initializer_list>
+#include <utility>
 
 using namespace ulmgpu;
 using namespace ulmgpu::xent;
@@ -495,7 +497,68 @@ int bad(const char *text)
 
 template <typename T> bool off(const void *p) { return (uintptr_t)p % sizeof(T) != 0; }
 
+// Memory that a call reads or writes: `columns` runs of `bytes`, `pitch` apart.
+struct Window {
+    uintptr_t at;
+    int64_t bytes, pitch, columns;
+    uintptr_t end() const { return at + (uintptr_t)((columns - 1) * pitch + bytes); }
+};
+template <typename T> Window matrix(const T *p, int rows, int columns, int ld)
+{
+    return {(uintptr_t)p, rows * (int64_t)sizeof(T), ld * (int64_t)sizeof(T), p ? columns : 0};
+}
+template <typename T> Window vector(const T *p, int64_t n)
+{
+    return {(uintptr_t)p, n * (int64_t)sizeof(T), n * (int64_t)sizeof(T), p && n > 0 ? 1 : 0};
+}
+
+// Whether two windows share a byte.  One may lie in the gaps between the other's columns (the halves of one wide matrix):
+// every column of the one with fewer of them that lies inside the other is compared with the two columns it can meet,
+// after a single comparison for all of them where the columns are equally far apart.
+bool meet(Window a, Window b)
+{
+    if (a.columns <= 0 || b.columns <= 0 || a.at >= b.end() || b.at >= a.end()) return false;
+    if (a.columns > b.columns) std::swap(a, b);
+    auto met = [&](uintptr_t from) {            // by a column of a
+        const int64_t k = from <= b.at ? 0 : std::min<int64_t>((int64_t)((from - b.at) / (uintptr_t)b.pitch), b.columns - 1);
+        for (int64_t i = k; i < std::min(k + 2, b.columns); ++i) {
+            const uintptr_t at = b.at + (uintptr_t)(i * b.pitch);
+            if (from < at + (uintptr_t)b.bytes && at < from + (uintptr_t)a.bytes) return true;
+        }
+        return false;
+    };
+    // the first column of a that ends behind b's beginning, the last one that begins before b's end
+    const int64_t first = a.at + (uintptr_t)a.bytes > b.at
+                              ? 0 : (int64_t)((b.at - a.at - (uintptr_t)a.bytes) / (uintptr_t)a.pitch) + 1;
+    const int64_t last = std::min(a.columns - 1, (int64_t)((b.end() - 1 - a.at) / (uintptr_t)a.pitch));
+    if (a.pitch == b.pitch) {
+        // columns between the ends meet what the ones before them met; at the ends a neighbour may be missing
+        return first <= last && (met(a.at + (uintptr_t)(first * a.pitch)) || met(a.at + (uintptr_t)(last * a.pitch)));
+    }
+    for (int64_t i = first; i <= last; ++i)
+        if (met(a.at + (uintptr_t)(i * a.pitch))) return true;
+    return false;
+}
+
+// Whether what a call writes (the first `written` windows) shares memory with anything else it is given.
+bool overlapping(std::initializer_list<Window> windows, int written)
+{
+    const Window *w = windows.begin();
+    const int n = (int)windows.size();
+    for (int i = 0; i < written; ++i)
+        for (int j = i + 1; j < n; ++j)
+            if (meet(w[i], w[j])) return true;
+    return false;
+}
+
 template <typename T> T *part_of(void *work, int64_t at) { return reinterpret_cast<T *>(static_cast<char *>(work) + at); }
+
+template <typename T> long worksize(int hidden, int tokens, int vocab, bool grad)
+{
+    if (!sizes_ok(hidden, tokens, vocab)) return 0;
+    if (grad && xent_takes_few(hidden, tokens)) return xent_few_worksize(hidden, tokens, vocab);
+    return (long)layout<T>(hidden, tokens, vocab, grad).bytes;
+}
 
 template <typename T>
 int xent_device(int hidden, int tokens, int vocab, float alpha, const T *W, int ldW, const T *X, int ldX,
@@ -510,6 +573,9 @@ int xent_device(int hidden, int tokens, int vocab, float alpha, const T *W, int 
         return bad("operand off its type's alignment");
     if ((uintptr_t)work & 15) return bad("workspace not on 16 bytes");
     const Layout l = layout<T>(hidden, tokens, vocab, false);
+    if (overlapping({vector(loss, tokens), vector(lse, tokens), vector(static_cast<char *>(work), l.bytes),
+                     matrix(W, hidden, vocab, ldW), matrix(X, hidden, tokens, ldX), vector(label, tokens)}, 3))
+        return bad("a result or the workspace overlaps another operand");
     TokenArgs t{};
     t.tokens = tokens;
     t.vocab = vocab;
@@ -588,6 +654,12 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
         off<float>(glse))
         return bad("operand off its type's alignment");
     if ((uintptr_t)work & 15) return bad("workspace not on 16 bytes");
+    // without tokens nothing but gW is touched
+    if (overlapping({matrix(gW, hidden, vocab, ldGW), matrix(gX, hidden, tokens, ldGX),
+                     vector(static_cast<char *>(work), worksize<T>(hidden, tokens, vocab, true)),
+                     matrix(W, hidden, tokens ? vocab : 0, ldW), matrix(X, hidden, tokens, ldX), vector(label, tokens),
+                     vector(lse, tokens), vector(gloss, tokens), vector(glse, tokens)}, 3))
+        return bad("a result or the workspace overlaps another operand");
     if (xent_takes_few(hidden, tokens))
         return xent_few_grad<T>(hidden, tokens, vocab, alpha, W, ldW, X, ldX, label, ignore, lse, gloss, glse, beta, gW, ldGW,
                                 gX, ldGX, static_cast<float *>(work), stream);
@@ -709,13 +781,6 @@ int xent_grad_device(int hidden, int tokens, int vocab, float alpha, const T *W,
         HIP_TRY(hipGetLastError());
     }
     return ULMBLAS_GPU_OK;
-}
-
-template <typename T> long worksize(int hidden, int tokens, int vocab, bool grad)
-{
-    if (!sizes_ok(hidden, tokens, vocab)) return 0;
-    if (grad && xent_takes_few(hidden, tokens)) return xent_few_worksize(hidden, tokens, vocab);
-    return (long)layout<T>(hidden, tokens, vocab, grad).bytes;
 }
 
 }  // namespace
