@@ -560,9 +560,9 @@ int ulmblas_gpu_bxent_grad(int hidden, int tokens, int vocab, float alpha,
  * group).  `work`: device memory of ulmblas_gpu_gnrm2_worksize(count) bytes,
  * 8-byte aligned, any contents, for one call at a time.
  * gclip: dY[i] = dX[i] * min(1, largest / *dNorm), elementwise, dNorm on the
- * device; dY[i] is dX[i] itself or does not overlap any tensor of the group, and
- * no two dY overlap (a tensor is in a group that is scaled in place once, else
- * BAD_ARGUMENT).
+ * device; dY[i] is dX[i] itself or does not overlap any tensor of the group, no
+ * two dY overlap (a tensor is in a group that is scaled in place once), and
+ * *dNorm is outside all dY (else BAD_ARGUMENT).
  * A norm that is infinite or no number leaves the values as they are.  Nothing
  * is allocated or synchronised; the same call gives the same bits. */
 long ulmblas_gpu_gnrm2_worksize(int count);

@@ -171,3 +171,22 @@ def test_overlapping_tensors_are_not_scaled():
     assert abs(float(blas.gpu_gnrm2([c, c])) - float(c.double().norm()) * 2 ** 0.5) < 1e-3
     blas.gpu_gclip([a, flat[32:48], c, flat[40:40]], norm, 0.5)
     assert (flat.cpu() == torch.arange(64) * 0.5).all()
+
+
+def test_a_norm_beside_and_inside_the_tensors():
+    """In a tensor that is read only, or next to one that is written, the norm may lie; inside one that is written not."""
+    import torch
+    flat = torch.full((40,), 2.0, device="cuda")
+    out = torch.empty(39, device="cuda")
+    a, norm = flat[:39], flat[39:]
+    blas.gpu_gnrm2([a], norm)
+    n = float(norm)
+    assert abs(n - 2 * 39 ** 0.5) <= 1.01 * U * n
+    blas.gpu_gclip([a], norm, 0.5 * n)              # next to it
+    assert (a == 1.0).all() and float(norm) == n
+    blas.gpu_gclip([flat[1:]], norm, 0.5 * n, out=[out])
+    assert (out[:38] == 0.5).all() and float(out[38]) == 0.5 * n and float(norm) == n
+    for tensors in ([flat], [flat[1:]], [a[:5], flat[39:]]):
+        with pytest.raises(blas.GpuError, match="norm"):
+            blas.gpu_gclip(tensors, norm, 0.5 * n)
+    assert (a == 1.0).all() and float(norm) == n

@@ -311,3 +311,12 @@ def test_windows_between_the_columns_of_others():
         assert got == meets, (H, T, V, ld, at)
         met += meets
     assert 200 < met < 1300         # both answers were asked for
+
+
+def test_clipping_refuses_a_norm_inside_a_tensor_it_writes():
+    """Some workgroups would read the norm after others have scaled it."""
+    for off in (0, 12):
+        for kw in (dict(x=(4096, 5000), y=(4096, 5000)), dict(x=(8192, 9000), y=(4096, 5000))):
+            assert group(which="clip", norm=C.c_void_p(4096 + off), **kw) == BAD, (off, kw)
+            assert b"overlaps" in lib.load().ulmblas_gpu_last_error()
+    assert group(which="clip", n=(0, 4), x=(None, 4096), y=(None, 4096), norm=C.c_void_p(4100)) == BAD

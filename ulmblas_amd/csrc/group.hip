@@ -212,9 +212,9 @@ int check(int count, const char *type, const long *n, const void *const *x)
     return ULMBLAS_GPU_OK;
 }
 
-// Whether the tensors written overlap neither each other nor any that is read, but for the one with the same number,
-// which may be the same memory.  (60 tensors: 1 us of the host's time.)
-int check_apart(int count, const char *type, const long *n, const void *const *x, void *const *y)
+// Whether the tensors written overlap neither each other nor the norm nor any that is read, but for the one with the same
+// number, which may be the same memory.  (60 tensors: 1 us of the host's time.)
+int check_apart(int count, const char *type, const long *n, const void *const *x, void *const *y, const float *norm)
 {
     struct Span {
         uintptr_t from, to;
@@ -222,10 +222,11 @@ int check_apart(int count, const char *type, const long *n, const void *const *x
     };
     std::vector<Span> spans;
     try {
-        spans.reserve(2 * (size_t)count);
+        spans.reserve(2 * (size_t)count + 1);
     } catch (const std::exception &) {
         return bad("out of host memory");
     }
+    spans.push_back({(uintptr_t)norm, (uintptr_t)(norm + 1), false});
     for (int i = 0; i < count; ++i) {
         if (n[i] == 0) continue;
         const uintptr_t bytes = (uintptr_t)n[i] * (type[i] == 's' ? 4 : 2), from = (uintptr_t)x[i], to = (uintptr_t)y[i];
@@ -235,7 +236,7 @@ int check_apart(int count, const char *type, const long *n, const void *const *x
     std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.from < b.from; });
     uintptr_t all = 0, written = 0;         // ends of the spans so far
     for (const Span &s : spans) {
-        if (s.from < (s.written ? all : written)) return bad("a tensor that is written overlaps another one");
+        if (s.from < (s.written ? all : written)) return bad("a tensor that is written overlaps another one or the norm");
         all = std::max(all, s.to);
         if (s.written) written = std::max(written, s.to);
     }
@@ -311,7 +312,7 @@ int ulmblas_gpu_gclip(int count, const char *type, const long *n, const void *co
     if (!(largest >= 0.0f)) return bad("largest norm negative or no number");
     if (count == 0) return ULMBLAS_GPU_OK;
     if (!dNorm) return bad("null norm");
-    if ((rc = check_apart(count, type, n, dX, dY))) return rc;
+    if ((rc = check_apart(count, type, n, dX, dY, dNorm))) return rc;
     GroupArgs g;
     for (int from = 0; from < count; from += kGroup) {
         const unsigned blocks = fill(g, from, count, type, n, dX, dY);
