@@ -558,7 +558,8 @@ int ulmblas_gpu_bxent_grad(int hidden, int tokens, int vocab, float alpha,
  * gnrm2: *dNorm = the Euclidean norm of all elements together (squares and
  * sums in fp64, so nothing overflows or underflows on the way; 0 for an empty
  * group).  `work`: device memory of ulmblas_gpu_gnrm2_worksize(count) bytes,
- * 8-byte aligned, any contents, for one call at a time.
+ * 8-byte aligned, any contents, for one call at a time, outside all dX (else
+ * BAD_ARGUMENT).
  * gclip: dY[i] = dX[i] * min(1, largest / *dNorm), elementwise, dNorm on the
  * device; dY[i] is dX[i] itself or does not overlap any tensor of the group, no
  * two dY overlap (a tensor is in a group that is scaled in place once), and

@@ -190,3 +190,16 @@ def test_a_norm_beside_and_inside_the_tensors():
         with pytest.raises(blas.GpuError, match="norm"):
             blas.gpu_gclip(tensors, norm, 0.5 * n)
     assert (a == 1.0).all() and float(norm) == n
+
+
+def test_a_workspace_beside_and_inside_the_tensors():
+    import torch
+    size = blas.gnrm2_worksize([None])
+    flat = torch.full((size // 4 + 200,), 1.0, device="cuda")
+    a = flat[:100]
+    assert float(blas.gpu_gnrm2([a], work=flat[100:])) == 10.0
+    assert (a == 1.0).all() and (flat[100 + size // 4:] == 1.0).all()
+    for work in (flat, flat[98:]):
+        with pytest.raises(blas.GpuError, match="workspace overlaps"):
+            blas.gpu_gnrm2([a], work=work)
+    assert (a == 1.0).all()

@@ -320,3 +320,12 @@ def test_clipping_refuses_a_norm_inside_a_tensor_it_writes():
             assert group(which="clip", norm=C.c_void_p(4096 + off), **kw) == BAD, (off, kw)
             assert b"overlaps" in lib.load().ulmblas_gpu_last_error()
     assert group(which="clip", n=(0, 4), x=(None, 4096), y=(None, 4096), norm=C.c_void_p(4100)) == BAD
+
+
+def test_norm_refuses_a_workspace_inside_a_tensor():
+    size, at = blas.gnrm2_worksize([None] * 2), 1 << 30
+    # the second tensor: 4 bf16 elements from `at` on, or long enough to reach into the workspace or around it
+    for kw in (dict(work=C.c_void_p(at)), dict(work=C.c_void_p(at + 8 - size)), dict(work=C.c_void_p(at + 4096), n=(4, 2049)),
+               dict(work=C.c_void_p(at + 4096), n=(4, 1 << 30))):
+        assert group(**{**dict(x=(1 << 40, at)), **kw}) == BAD, kw
+        assert b"workspace overlaps" in lib.load().ulmblas_gpu_last_error(), kw

@@ -287,6 +287,12 @@ int ulmblas_gpu_gnrm2(int count, const char *type, const long *n, const void *co
     if (rc) return rc;
     if (!dNorm || !work) return bad("null result or workspace");
     if ((uintptr_t)work & 7) return bad("workspace not on 8 bytes");
+    const uintptr_t from = (uintptr_t)work, to = from + (uintptr_t)ulmblas_gpu_gnrm2_worksize(count);
+    for (int i = 0; i < count; ++i) {
+        const uintptr_t x = (uintptr_t)dX[i];
+        if (n[i] > 0 && x < to && from < x + (uintptr_t)n[i] * (type[i] == 's' ? 4 : 2))
+            return bad("the workspace overlaps a tensor");
+    }
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     double *partial = static_cast<double *>(work);
     int sums = 0;
