@@ -203,3 +203,22 @@ def test_a_workspace_beside_and_inside_the_tensors():
         with pytest.raises(blas.GpuError, match="workspace overlaps"):
             blas.gpu_gnrm2([a], work=work)
     assert (a == 1.0).all()
+
+
+def test_tensors_whose_memory_was_replaced():
+    import torch
+    x, y = torch.full((100,), 3.0, device="cuda"), torch.full((100,), 4.0, device="cuda")
+    group = blas.TensorGroup([x, y])
+    assert float(blas.gpu_gnrm2(group)) == 50.0
+    old = x.data
+    x.data = torch.zeros(100, device="cuda")
+    norm = torch.full((1,), 50.0, device="cuda")
+    with pytest.raises(ValueError, match="tensor 0 was replaced"):
+        blas.gpu_gnrm2(group)
+    with pytest.raises(ValueError, match="tensor 0 was replaced"):
+        blas.gpu_gclip(group, norm, 25.0)
+    assert (old == 3.0).all() and (y == 4.0).all()
+    assert float(blas.gpu_gnrm2(blas.TensorGroup([x, y]))) == 40.0
+    x.data = old                        # back again
+    blas.gpu_gclip(group, norm, 25.0)
+    assert (x == 1.5).all() and (y == 2.0).all()

@@ -183,6 +183,7 @@ class FakeStreams:
                             ("ExternalStream", Stream), ("default_stream", lambda *a: default), ("stream", Inside),
                             ("is_current_stream_capturing", lambda: fake.now in captured)):
             monkeypatch.setattr(torch.cuda, name, value)
+        monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: fake.now)
         monkeypatch.setattr(torch, "empty", empty)
         monkeypatch.setattr(torch, "zeros", empty)
         self.device = torch.device("cuda", 0)
@@ -329,3 +330,29 @@ def test_norm_refuses_a_workspace_inside_a_tensor():
                dict(work=C.c_void_p(at + 4096), n=(4, 1 << 30))):
         assert group(**{**dict(x=(1 << 40, at)), **kw}) == BAD, kw
         assert b"workspace overlaps" in lib.load().ulmblas_gpu_last_error(), kw
+
+
+def test_a_group_whose_memory_was_replaced_is_refused(monkeypatch):
+    """Its addresses are those of memory that may belong to others by now."""
+    torch = pytest.importorskip("torch")
+    monkeypatch.setattr(blas, "_device_of", lambda named: None)
+
+    def make():
+        tensors = [torch.ones(5), torch.ones(7, dtype=torch.bfloat16), torch.ones(9)]
+        return tensors, blas.TensorGroup(tensors)
+
+    norm = torch.ones(1)
+    tensors, group = make()
+    group.check()
+    tensors[1].fill_(3.0)               # other values in the same memory are no other memory
+    group.check()
+    tensors[1].data = torch.ones(7, dtype=torch.bfloat16)
+    tensors2, resized = make()
+    tensors2[2].resize_(1 << 20)
+    tensors3, released = make()
+    tensors3[0].untyped_storage().resize_(0)
+    for g, i in ((group, 1), (resized, 2), (released, 0)):
+        for call in (lambda: blas.gpu_gnrm2(g), lambda: blas.gpu_gclip(g, norm, 1.0),
+                     lambda: blas.gpu_gclip(make()[1], norm, 1.0, out=g), lambda: blas.gpu_gclip(g, norm, 1.0, out=make()[1])):
+            with pytest.raises(ValueError, match=f"tensor {i} was replaced"):
+                call()
