@@ -356,3 +356,18 @@ def test_a_group_whose_memory_was_replaced_is_refused(monkeypatch):
                      lambda: blas.gpu_gclip(make()[1], norm, 1.0, out=g), lambda: blas.gpu_gclip(g, norm, 1.0, out=make()[1])):
             with pytest.raises(ValueError, match=f"tensor {i} was replaced"):
                 call()
+
+
+def test_ignore_beyond_32_bits_is_refused():
+    """As a C int 2^32 + 3 would be 3, and the tokens of row 3 would lose their target."""
+    torch = pytest.importorskip("torch")
+    W, X, f = torch.zeros(10, 8), torch.zeros(4, 8), torch.zeros(4)
+    label = torch.zeros(4, dtype=torch.int32)
+    for ignore in ((1 << 32) + 3, 1 << 31, -(1 << 31) - 1):
+        with pytest.raises(ValueError, match="32-bit"):
+            blas.gpu_xent("s", 8, 4, 10, 1.0, W, 8, X, 8, label, ignore)
+        with pytest.raises(ValueError, match="32-bit"):
+            blas.gpu_xent_grad("s", 8, 4, 10, 1.0, W, 8, X, 8, label, ignore, f, f, None, 0.0, None, 8, None, 8)
+    for ignore in ((1 << 31) - 1, -(1 << 31)):          # these go on to what is wrong with the operands
+        with pytest.raises(ValueError, match="not on a GPU"):
+            blas.gpu_xent("s", 8, 4, 10, 1.0, W, 8, X, 8, label, ignore)

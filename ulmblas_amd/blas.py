@@ -549,6 +549,12 @@ def _window(what, prec, x, rows, cols, ld):
     _fits(what, prec, x, rows, cols, ld)
 
 
+def _int32(what, value):
+    """A value that the library takes as a C int; ctypes would drop what is beyond."""
+    if not -(1 << 31) <= value < 1 << 31:
+        raise ValueError(f"{what}: {value} is no 32-bit value")
+
+
 def _vector(what, x, n, dtype):
     if x is None:
         return
@@ -583,6 +589,7 @@ def gpu_xent(prec, hidden, tokens, vocab, alpha, dW, ldW, dX, ldX, dLabel, ignor
     or no row of the classifier have loss and lse 0.  Returns (dLoss, dLse), float32, allocated unless given.
     Asynchronous; a `stream` (raw hipStream_t value) other than torch's current one waits for the current one first."""
     import torch
+    _int32("ignore", ignore)
     _window("W", prec, dW, hidden, vocab, ldW)
     _window("X", prec, dX, hidden, tokens, ldX)
     _vector("labels", dLabel, tokens, torch.int32)
@@ -606,6 +613,7 @@ def gpu_xent_grad(prec, hidden, tokens, vocab, alpha, dW, ldW, dX, ldX, dLabel, 
     dGX (hidden x tokens) and dGW (hidden x vocab, alpha * X * P^T + beta * dGW) take the operands' type; None leaves
     one out.  Returns (dGW, dGX).  Asynchronous; `stream` as for gpu_xent."""
     import torch
+    _int32("ignore", ignore)
     for name, x, cols, ld in (("W", dW, vocab, ldW), ("X", dX, tokens, ldX), ("gW", dGW, vocab, ldGW),
                               ("gX", dGX, tokens, ldGX)):
         _window(name, prec, x, hidden, cols, ld)
