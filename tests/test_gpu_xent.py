@@ -591,3 +591,23 @@ def test_gradients_between_the_rows_of_the_operands(prec, tokens):
                                wide.view(-1)[off:], 2 * H, None, H)
     with pytest.raises(blas.GpuError, match="overlaps"):
         blas.gpu_xent(prec, H, T, V, 1.0, p.W, p.ldW, p.X, p.ldX, p.dlabel, IGNORE, both[:T], both[T - 1:2 * T - 1])
+
+
+@pytest.mark.parametrize("prec", ["s", "b"])
+@pytest.mark.parametrize("pad", [0, 1])
+def test_nothing_behind_the_workspace_is_written(prec, pad):
+    """Vocabularies that end in every part of a tile, on both sides of the sizes at which the tiles change."""
+    import torch
+    for tokens in (1, 32, 33, 257, 600):
+        for vocab in (1, 127, 129, 257, 1025, 2000):
+            p = Problem(prec, 72, tokens, vocab, pad=pad, seed=tokens + vocab)
+            sizes = [f(prec, 72, tokens, vocab) for f in (blas.xent_worksize, blas.xent_grad_worksize)]
+            works = [torch.full((size + 4096,), 0x5a, dtype=torch.uint8, device="cuda") for size in sizes]
+            gW, gX = (torch.empty(n, 72, dtype=p.W.dtype, device="cuda") for n in (vocab, tokens))
+            loss, lse = blas.gpu_xent(prec, 72, tokens, vocab, 1.0, p.W, p.ldW, p.X, p.ldX, p.dlabel, work=works[0])
+            blas.gpu_xent_grad(prec, 72, tokens, vocab, 1.0, p.W, p.ldW, p.X, p.ldX, p.dlabel, IGNORE, lse,
+                               torch.ones(tokens, device="cuda"), None, 0.0, gW, 72, gX, 72, work=works[1])
+            torch.cuda.synchronize()
+            for work, size in zip(works, sizes):
+                assert (work[size:] == 0x5a).all(), (tokens, vocab)
+            p.check_forward()

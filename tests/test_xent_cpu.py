@@ -371,3 +371,16 @@ def test_ignore_beyond_32_bits_is_refused():
     for ignore in ((1 << 31) - 1, -(1 << 31)):          # these go on to what is wrong with the operands
         with pytest.raises(ValueError, match="not on a GPU"):
             blas.gpu_xent("s", 8, 4, 10, 1.0, W, 8, X, 8, label, ignore)
+
+
+@pytest.mark.parametrize("p", ["s", "b"])
+def test_workspace_of_the_forward_call(p):
+    """8 bytes for every token and 128 rows of W, a copy of X (in steps of 128 bytes), for bf16 at most 128 MiB of
+    packed W, and 16 bytes a token (tokens in 256s)."""
+    size = {"s": 4, "b": 2}[p]
+    for hidden, tokens, vocab in ((4096, 8192, 131072), (64, 1 << 20, 131072), (1000, 333, 20011), (8, 40, 300)):
+        tp, hp = -(-tokens // 256) * 256, -(-hidden // (128 // size)) * 128
+        packed = (1 << 27 if p == "b" else 0) + 256 * hp
+        assert blas.xent_worksize(p, hidden, tokens, vocab) <= tp * (-(-vocab // 256) * 16 + hp + 16) + packed + 2048
+    # what the tiles of 64 rows need, which bf16 takes up to 32 tokens where W lies off words
+    assert blas.xent_worksize("b", 64, 32, 1 << 20) >= 256 * (1 << 20) // 64 * 8

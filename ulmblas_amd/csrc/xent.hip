@@ -406,7 +406,8 @@ struct Layout {
     int64_t rows, label, place, lse, both, gloss, delta, target, bucket, member, rank, count, x, w, stats, p, part, bytes;
 };
 
-// of P and of a packed copy of W in the gradient, and of a packed copy of W in the forward call, at the most
+// of P and of a packed copy of W in the gradient, and of a packed copy of W in the forward call, at the most (where 256
+// rows are not more)
 constexpr int64_t kPieceBytes = (int64_t)1 << 30, kPackBytes = (int64_t)1 << 27;
 
 template <typename T> Layout layout(int hidden, int tokens, int vocab, bool grad)
@@ -444,7 +445,9 @@ template <typename T> Layout layout(int hidden, int tokens, int vocab, bool grad
     l.x = take(l.tokens_p * l.hidden_p * (int64_t)sizeof(T));
     l.w = take(packs ? (int64_t)l.piece * l.hidden_p * (int64_t)sizeof(T) : 0);
     if (!grad) {
-        l.stats = take((round_up(vocab, 256) / kAnyTile.rows) * l.tokens_p * 8);
+        // a tile has 128 rows at least, but for few tokens of bf16, whose W may lie off words
+        const int rows = sizeof(T) == 2 && tokens <= kNarrow ? kAnyTile.rows : kTiles[1].rows;
+        l.stats = take((round_up(vocab, 256) / rows) * l.tokens_p * 8);
     } else {
         l.p = take(l.tokens_p * l.piece * (int64_t)sizeof(T));
         // as many splits as fill kGroups workgroups with tiles, or one
