@@ -523,15 +523,16 @@ int ulmblas_gpu_bxent(int hidden, int tokens, int vocab, float alpha,
                       int ignore, float *dLoss, float *dLse, void *work,
                       void *stream);
 /* The gradient of the above.  dLse is what the forward call returned, dGLoss
- * and dGLse (null: zero) the gradients of its two results; with
+ * the gradient of its loss and dGLse (null: zero) that of its lse; with
  *     P_vt = dGLoss[t] (exp(z_vt - dLse[t]) - [v = label]) + dGLse[t] exp(z_vt - dLse[t])
  * for tokens with a target and 0 for others,
  *     gX = alpha * W * P            (hidden x tokens; whole columns are written)
  *     gW = alpha * X * P^T + beta * gW      (hidden x vocab)
  * beta == 0 never reads gW.  A null dGW or dGX is not computed.  The logits are
  * computed again, a piece of the vocabulary at a time, and P of that piece is
- * rounded to the operands' type for the two products (up to 8 tokens it is not:
- * hidden up to 4096, or 8192 with up to 4 tokens).  dGW, dGX and `work`
+ * rounded to the operands' type for the two products, but for what rounding
+ * takes at the labels (up to 8 tokens it is not rounded: hidden up to 4096, or
+ * 8192 with up to 4 tokens).  dGW, dGX and `work`
  * (ulmblas_gpu_?xent_grad_worksize bytes) share no memory with each other or
  * the operands (BAD_ARGUMENT); the columns of one matrix may lie between those
  * of another. */
@@ -560,11 +561,12 @@ int ulmblas_gpu_bxent_grad(int hidden, int tokens, int vocab, float alpha,
  * group).  `work`: device memory of ulmblas_gpu_gnrm2_worksize(count) bytes,
  * 8-byte aligned, any contents, for one call at a time, outside all dX (else
  * BAD_ARGUMENT).
- * gclip: dY[i] = dX[i] * min(1, largest / *dNorm), elementwise, dNorm on the
- * device; dY[i] is dX[i] itself or does not overlap any tensor of the group, no
- * two dY overlap (a tensor is in a group that is scaled in place once), and
- * *dNorm is outside all dY (else BAD_ARGUMENT).
- * A norm that is infinite or no number leaves the values as they are.  Nothing
+ * gclip: dY[i] = dX[i] * f, elementwise, with f = min(1, largest / *dNorm), or
+ * 1 where the norm is infinite or no number: such values stay as they are, and
+ * so do finite ones whose norm is beyond fp32's range (*dNorm shows it).  dNorm
+ * is on the device; dY[i] is dX[i] itself or does not overlap any tensor of the
+ * group, no two dY overlap (a tensor is in a group that is scaled in place
+ * once), and *dNorm is outside all dY (else BAD_ARGUMENT).  Nothing
  * is allocated or synchronised; the same call gives the same bits. */
 long ulmblas_gpu_gnrm2_worksize(int count);
 int ulmblas_gpu_gnrm2(int count, const char *type, const long *n,

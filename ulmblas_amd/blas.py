@@ -609,7 +609,7 @@ def gpu_xent(prec, hidden, tokens, vocab, alpha, dW, ldW, dX, ldX, dLabel, ignor
 
 def gpu_xent_grad(prec, hidden, tokens, vocab, alpha, dW, ldW, dX, ldX, dLabel, ignore, dLse, dGLoss, dGLse, beta, dGW,
                   ldGW, dGX, ldGX, work=None, stream=None):
-    """Gradient of gpu_xent: dLse is its second result, dGLoss and dGLse (None: zero) the gradients of its results.
+    """Gradient of gpu_xent: dLse is its second result, dGLoss the gradient of its loss, dGLse (None: zero) that of lse.
     dGX (hidden x tokens) and dGW (hidden x vocab, alpha * X * P^T + beta * dGW) take the operands' type; None leaves
     one out.  Returns (dGW, dGX).  Asynchronous; `stream` as for gpu_xent."""
     import torch
@@ -635,7 +635,7 @@ def gpu_xent_grad(prec, hidden, tokens, vocab, alpha, dW, ldW, dX, ldX, dLabel, 
 class TensorGroup:
     """A list of float32 / bfloat16 tensors on one GPU as gpu_gnrm2 and gpu_gclip take it: the lists of addresses,
     lengths and types are made once.  A program that passes the same tensors again keeps one; the group keeps its
-    tensors, and tensors whose memory is replaced need a new group: calls refuse the old one (30 tensors: 3 us)."""
+    tensors, and tensors whose memory is replaced need a new group: calls refuse the old one (30 tensors: 1.2 us)."""
 
     def __init__(self, tensors):
         import torch
@@ -692,9 +692,10 @@ def gpu_gnrm2(tensors, dNorm=None, work=None, stream=None):
 
 
 def gpu_gclip(tensors, dNorm, largest, out=None, stream=None):
-    """Multiplies a TensorGroup (or list of tensors) by min(1, largest / dNorm), in place or into the TensorGroup (or
-    list) `out` of the same lengths and types; returns the group that was written.  No tensor that is written may
-    overlap another one (a group of the same tensor twice is refused).  Asynchronous; `stream` as for gpu_xent."""
+    """Multiplies a TensorGroup (or list of tensors) by min(1, largest / dNorm), or by 1 where the norm is infinite or no
+    number, in place or into the TensorGroup (or list) `out` of the same lengths and types; returns the group that was
+    written.  No tensor that is written may overlap another one or the norm (a group of the same tensor twice is
+    refused).  Asynchronous; `stream` as for gpu_xent."""
     import torch
     g = _as_group(tensors)
     o = g if out is None or out is g else _as_group(out)

@@ -31,12 +31,12 @@
 // takes is 8 KB at a time (rows of P 128 KB apart: 3.53 ms for the GX product
 // 4096 x 8192 x 65536, in blocks 3.32 ms).
 //
-// Measured on bf16 tiles of 256 x 256, K = 65536 (GX) and 4096 (STATS): the
-// matrix cores are busy 57 - 70 % of the time at the 1.8 - 2.1 GHz that the power
-// limit leaves.  With the fetches left out the same loop runs 25 % faster,
-// with all of them served by L2 10 % faster; more steps in flight (up to 2) do
-// not help.  16 x 16 MFMAs run at a higher clock than 32 x 32 ones (they read
-// and write half the accumulators per product): STATS 1.90 -> 1.81 ms.
+// Measured on bf16 tiles of 256 x 256 (tokens x hidden x vocabulary): the matrix
+// cores are busy 58 - 66 % of the cycles on 8192 x 4096 x 131072 and 35 - 57 % on
+// 2048 x 2048 x 32768, half masked (GW the least: 16 steps a tile), at the 1.5 -
+// 2.1 GHz that the power limit leaves.  16 x 16 MFMAs run at a higher clock than
+// 32 x 32 ones (they read and write half the accumulators per product): STATS
+// 1.90 -> 1.81 ms (8192 x 4096 x 32768).
 #ifndef ULMBLAS_XENT_KERNEL_HIP_H
 #define ULMBLAS_XENT_KERNEL_HIP_H 1
 
@@ -775,9 +775,11 @@ __device__ void Product<T, MODE, BM, BN, WM, WN, BUFFERS, ANY>::run(const Produc
         }
     } else if constexpr (MODE == PROB) {
         // P is rounded to the operands' type, since the two products that follow run on it: each element is off
-        // by at most half a step of that type, and the sums over tokens or vocabulary average that out - except
-        // at the label, whose element outweighs the others: what its rounding took is kept (bf16) and goes into
-        // both products in fp32.  Past the last token and the last vocabulary row the tile is zeros, which the
+        // by at most half a step of that type (bf16: 2^-8 of itself), and the sums over tokens or vocabulary
+        // average that out - except at the label, whose element mostly outweighs the others: what its rounding
+        // took is kept (bf16) and goes into both products in fp32.  Elsewhere it stays: a row of gW that is
+        // nobody's label, and a token whose softmax lies on another row than its label's, have it on top of the
+        // result's own rounding.  Past the last token and the last vocabulary row the tile is zeros, which the
         // products may run into.
         unsigned char *P = static_cast<unsigned char *>(g.P);
         const float scale = scale_of<T>(g.alpha);
